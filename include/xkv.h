@@ -277,6 +277,101 @@ XKV_API int xkv_latent_append(const void* x, int64_t x_sb, const void* proj, int
 XKV_API int xkv_peer_allgather(const void* local, size_t shard_bytes, void* const* bufs, size_t flags_offset, int rank,
                        int world, uint32_t epoch, int* status_dev, void* stream);
 
+/*
+ * Rotary positions for queries and keys of new tokens, in one launch.  Token t of sequence b sits at position
+ *   positions == NULL           position + t
+ *   positions, pos_st == 0      positions[b * pos_sb] + t          (consecutive tokens)
+ *   positions, pos_st != 0      positions[b * pos_sb + t * pos_st] (drafted tokens, packed prompts)
+ * and pair j of its first rotary_dim elements turns by angle position * inv_freq[j]:
+ *   (a, b) -> magnitude * (a cos - b sin, b cos + a sin)
+ * with the pair at (j, j + rotary_dim / 2), or at (2j, 2j + 1) when `interleaved`.  Elements from rotary_dim on are
+ * copied.  inv_freq is fp64 (device, rotary_dim / 2 entries): the angle is reduced to one turn in fp64, so it keeps
+ * full fp32 accuracy at any int32 position.  q (batch, num_heads, num_tokens, head_dim), k the same with
+ * num_kv_heads; k == NULL (num_kv_heads 0) rotates queries only.  Outputs may be the inputs themselves (same
+ * pointer and strides); any other overlap is not supported.  xkv_rope_query is the one-token, whole-head form
+ * that shares the key-reconstruction kernels' fp32 angles.
+ */
+typedef struct xkv_rotary_params {
+  int32_t dtype, batch, num_heads, num_kv_heads, num_tokens, head_dim, rotary_dim, interleaved;
+  int32_t position;
+  float magnitude;
+  const int32_t* positions; int64_t pos_sb, pos_st;
+  const double* inv_freq;
+  const void* q; int64_t q_sb, q_sh, q_st;
+  const void* k; int64_t k_sb, k_sh, k_st;
+  void* q_out;   int64_t qo_sb, qo_sh, qo_st;
+  void* k_out;   int64_t ko_sb, ko_sh, ko_st;
+} xkv_rotary_params;
+XKV_API size_t xkv_rotary_params_size(void);
+XKV_API int xkv_rotary(const xkv_rotary_params* p, void* stream);
+
+/*
+ * Key / value caches held in 8 bits.  A cache row (one token of one KV head, head_dim elements) is head_dim codes and
+ * one fp32 scale: value = code * scale.  With top the row's largest magnitude and C the largest code (127, or 448
+ * for e4m3): scale = top * (1 / C) and code = round-to-nearest-even(x * (C * (1 / top))) clamped to +-C, every
+ * operation rounded to fp32.  A row whose scale would be below 2^-126 is held as zeros (scale 0); a row that holds an infinity or a NaN gets codes 0
+ * and a NaN scale, so that it reads back as NaN throughout instead of as plausible numbers.
+ *   codes  (batch, num_kv_heads, capacity, head_dim), 1 byte each, innermost contiguous
+ *   scales (batch, num_kv_heads, capacity) fp32, innermost contiguous
+ */
+typedef enum xkv_cache_code { XKV_CACHE_DENSE = 0, XKV_CACHE_INT8 = 1, XKV_CACHE_E4M3 = 2 } xkv_cache_code;
+
+/*
+ * xkv_cache_append writes num_tokens rows per sequence: token t of k / v (batch, num_kv_heads, num_tokens, head_dim)
+ * of `dtype` goes to cache row start_b + t, where start_b = positions ? positions[b] : position.  With `lengths`
+ * (device int32, batch entries) only the first min(lengths[b], num_tokens) tokens of sequence b are written.
+ * xkv_cache_read writes code * scale of cache rows start_b + t to k / v.  Cache rows outside [0, capacity) are
+ * left alone by the append and read as zeros by the read; `lengths` is the append's alone.  head_dim <= 1024.
+ */
+typedef struct xkv_cache_params {
+  int32_t dtype, cache_code, batch, num_kv_heads, num_tokens, capacity, head_dim;
+  int32_t position;
+  const int32_t* positions;
+  const int32_t* lengths;
+  void* k; int64_t k_sb, k_sh, k_st;
+  void* v; int64_t v_sb, v_sh, v_st;
+  void* k_codes; int64_t kc_sb, kc_sh, kc_sl;
+  void* v_codes; int64_t vc_sb, vc_sh, vc_sl;
+  float* k_scales; int64_t ks_sb, ks_sh;
+  float* v_scales; int64_t vs_sb, vs_sh;
+} xkv_cache_params;
+XKV_API size_t xkv_cache_params_size(void);
+XKV_API int xkv_cache_append(const xkv_cache_params* p, void* stream);
+XKV_API int xkv_cache_read(const xkv_cache_params* p, void* stream);
+
+/*
+ * Attention of num_tokens query tokens per sequence (1: plain decode; more: a drafted chain or tree) over a dense
+ * or an 8-bit cache.  Sequence b uses its first len_b = min(kv_lens[b], kv_len) cache rows (kv_lens NULL: kv_len).  The
+ * last num_tokens of them are the drafted tokens themselves, already written: token u sits in row
+ * len_b - num_tokens + u (tokens whose row would be negative are absent).  Token t sees every row in front of the
+ * drafted ones, and drafted token u where tree_mask[b * tm_sb + t * tm_st + u] != 0 (tree_mask NULL: u <= t).
+ * What a token does not see contributes nothing, whatever its row holds; a token that sees nothing gives zeros.
+ *   q   (batch, num_heads, num_tokens, head_dim) of dtype
+ *   k,v (batch, num_kv_heads, kv_len, head_dim): of dtype (XKV_CACHE_DENSE), or codes with k_scales / v_scales
+ *   out (batch, num_heads * num_tokens, head_dim) of dtype: row h * num_tokens + t at o_sb, o_sr
+ * Flags: XKV_FLAG_FORCE_GENERIC.  head_dim <= 256.  The status words at the start of the workspace are read with
+ * xkv_workspace_status, as for xkv_decode.
+ */
+typedef struct xkv_tree_params {
+  int32_t dtype, cache_code;
+  uint32_t flags;
+  int32_t batch, num_heads, num_kv_heads, num_tokens, kv_len, head_dim;
+  int32_t num_splits;  /* KV-split hint, 0 = choose */
+  float sm_scale;
+  const int32_t* kv_lens;
+  const uint8_t* tree_mask; int64_t tm_sb, tm_st;
+  const void* q; int64_t q_sb, q_sh, q_st;
+  const void* k; int64_t k_sb, k_sh, k_sl;
+  const void* v; int64_t v_sb, v_sh, v_sl;
+  const float* k_scales; int64_t ks_sb, ks_sh;
+  const float* v_scales; int64_t vs_sb, vs_sh;
+  void* out; int64_t o_sb, o_sr;
+} xkv_tree_params;
+XKV_API size_t xkv_tree_params_size(void);
+XKV_API const char* xkv_tree_decode_plan(const xkv_tree_params* p);
+XKV_API size_t xkv_tree_decode_workspace_bytes(const xkv_tree_params* p);
+XKV_API int xkv_tree_decode(const xkv_tree_params* p, void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -7,6 +7,7 @@ from __future__ import annotations
 
 import ctypes as C
 import os
+import struct
 import threading
 
 import torch
@@ -27,7 +28,18 @@ EXPORTS = [
     "xkv_dense_decode", "xkv_absorbed_decode", "xkv_recon_rope_decode", "xkv_qab_logits",
     "xkv_mla_decode", "xkv_group_decode_workspace_bytes", "xkv_group_decode", "xkv_merge",
     "xkv_rope_table", "xkv_rope_query", "xkv_latent_append", "xkv_peer_allgather",
+    "xkv_rotary_params_size", "xkv_rotary", "xkv_cache_params_size", "xkv_cache_append", "xkv_cache_read",
+    "xkv_tree_params_size", "xkv_tree_decode_plan", "xkv_tree_decode_workspace_bytes", "xkv_tree_decode",
 ]
+
+# Parameter blocks of the per-token operators, packed in the field order of include/xkv.h (native alignment; the sizes are
+# compared with the library's when it is loaded).  A packed call costs a tenth of filling a ctypes.Structure, which is
+# what a launch-bound call of a few microseconds notices.
+ROTARY_PARAMS = struct.Struct("@9if" + "P2q" + "P" + "P3q" * 4)
+CACHE_PARAMS = struct.Struct("@8i" + "PP" + "P3q" * 4 + "P2q" * 2)
+TREE_PARAMS = struct.Struct("@2iI6iif" + "P" + "P2q" + "P3q" * 3 + "P2q" * 2 + "P2q")
+CACHE_DENSE, CACHE_INT8, CACHE_E4M3 = 0, 1, 2
+CACHE_CODES = {torch.int8: CACHE_INT8, torch.float8_e4m3fn: CACHE_E4M3}
 
 
 class DecodeParams(C.Structure):
@@ -118,6 +130,22 @@ def load():
         lib.xkv_decode_builtin_scratch.argtypes = [C.POINTER(DecodeParams), C.c_void_p]
         lib.xkv_workspace_status.restype = C.c_int
         lib.xkv_workspace_status.argtypes = [C.c_void_p, C.c_void_p, C.POINTER(C.c_int32)]
+        for name in ("xkv_rotary", "xkv_cache_append", "xkv_cache_read"):
+            fn = getattr(lib, name)
+            fn.restype = C.c_int
+            fn.argtypes = [C.c_char_p, C.c_void_p]
+        lib.xkv_tree_decode_plan.restype = C.c_char_p
+        lib.xkv_tree_decode_plan.argtypes = [C.c_char_p]
+        lib.xkv_tree_decode_workspace_bytes.restype = C.c_size_t
+        lib.xkv_tree_decode_workspace_bytes.argtypes = [C.c_char_p]
+        lib.xkv_tree_decode.restype = C.c_int
+        lib.xkv_tree_decode.argtypes = [C.c_char_p, C.c_void_p, C.c_size_t, C.c_void_p]
+        for name, block in (("xkv_rotary_params_size", ROTARY_PARAMS), ("xkv_cache_params_size", CACHE_PARAMS),
+                            ("xkv_tree_params_size", TREE_PARAMS)):
+            fn = getattr(lib, name)
+            fn.restype = C.c_size_t
+            if fn() != block.size:
+                raise RuntimeError(f"{name[:-5]} layout differs between libxkv.so and its packed form")
         if lib.xkv_version() != 1:
             raise RuntimeError("libxkv.so version mismatch")
         if lib.xkv_decode_params_size() != C.sizeof(DecodeParams):
@@ -232,6 +260,40 @@ def run_decode(params: DecodeParams, device: torch.device, entry: str = "xkv_dec
         check(rc, entry)
         if _check_status if check_status is None else check_status:
             raise_on_status(ws.data_ptr(), stream, entry)
+
+
+def launch(fn: str, block: bytes, device: torch.device):
+    """Run entry point `fn` (a packed parameter block and the stream) on `device`'s current stream."""
+    lib = load()
+    idx = _device_of(device)
+    if idx == torch.cuda.current_device():
+        rc = getattr(lib, fn)(block, torch._C._cuda_getCurrentRawStream(idx))
+    else:
+        with torch.cuda.device(idx):
+            rc = getattr(lib, fn)(block, torch._C._cuda_getCurrentRawStream(idx))
+    if rc:
+        check(rc, fn)
+
+
+def run_tree_decode(block: bytes, device: torch.device, check_status=None):
+    """xkv_tree_decode with a workspace of the call's own: the caching allocator hands it on in stream order, and a
+    captured call keeps its workspace in its graph's pool, so no two graphs or streams share one."""
+    idx = _device_of(device)
+    if idx != torch.cuda.current_device():
+        with torch.cuda.device(idx):
+            return run_tree_decode(block, device, check_status)
+    lib = load()
+    nbytes = lib.xkv_tree_decode_workspace_bytes(block)
+    if nbytes == 0:
+        # let the entry point produce the precise status
+        check(lib.xkv_tree_decode(block, None, 0, None) or -2, "xkv_tree_decode")
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
+    stream = torch._C._cuda_getCurrentRawStream(idx)
+    rc = lib.xkv_tree_decode(block, ws.data_ptr(), nbytes, stream)
+    if rc:
+        check(rc, "xkv_tree_decode")
+    if _check_status if check_status is None else check_status:
+        raise_on_status(ws.data_ptr(), stream, "xkv_tree_decode")
 
 
 def last_status(device: torch.device):

@@ -19,7 +19,16 @@ from .attention import (  # noqa: F401
     xkv_group_decode,
     xkv_group_decode_v_only,
     mla_absorbed_decode,
+    group_query_attention_quantized,
+    group_query_attention_tree,
 )
+from .quant_cache import (  # noqa: F401
+    QuantizedCache,
+    quantized_cache,
+    quantized_cache_append,
+    quantized_cache_read,
+)
+from .rotary import rotary_embedding, rotary_frequencies  # noqa: F401
 from . import flash_recontruction, flash_decoding  # noqa: F401
 
 __version__ = "0.1.0"

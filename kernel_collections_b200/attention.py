@@ -16,7 +16,7 @@ from __future__ import annotations
 
 import torch
 
-from . import _C, ops
+from . import _C, ops, quant_cache
 
 
 def _no_mask(attn_mask, dropout_p):
@@ -283,6 +283,81 @@ def latent_append(latent, new_rows, proj, position):
                                          b, x.shape[1], R, cap, torch.cuda.current_stream(latent.device).cuda_stream)
     _C.check(rc, "xkv_latent_append")
     return latent
+
+
+def _tree_decode(query, k, v, k_scales, v_scales, code, tree_mask, sm_scale, kv_lens, num_splits, force_generic,
+                 check_status):
+    """Shared by the two tree entry points: k / v (bsz, num_kv_heads, kv_len, head_dim), scales or None."""
+    b, H, T, D = query.shape
+    KVH, L = k.shape[1], k.shape[2]
+    if H % KVH != 0:
+        raise ValueError("num_heads must be divisible by num_kv_heads")
+    tm_ptr, tm_sb, tm_st = 0, 0, 0
+    if tree_mask is not None:
+        _C.require_cuda(query, tree_mask)
+        if tree_mask.dtype != torch.bool or tuple(tree_mask.shape) not in ((T, T), (b, T, T)):
+            raise ValueError(f"tree_mask must be a bool tensor of shape ({T}, {T}) or ({b}, {T}, {T}); got "
+                             f"{tree_mask.dtype} {tuple(tree_mask.shape)}")
+        if tree_mask.stride(-1) != 1 and T != 1:
+            tree_mask = tree_mask.contiguous()
+        tm_ptr, tm_st = tree_mask.data_ptr(), tree_mask.stride(-2)
+        tm_sb = tree_mask.stride(0) if tree_mask.dim() == 3 else 0
+    len_ptr = 0
+    if kv_lens is not None:
+        _C.require_cuda(query, kv_lens)
+        if kv_lens.dtype != torch.int32 or tuple(kv_lens.shape) != (b,) or not kv_lens.is_contiguous():
+            raise ValueError("kv_lens must be a contiguous int32 tensor of shape (batch,)")
+        len_ptr = kv_lens.data_ptr()
+    q = query if query.stride(3) == 1 or D == 1 else query.contiguous()
+    out = torch.empty((b, H, T, D), dtype=q.dtype, device=q.device)
+    qs, ks, vs = q.stride(), k.stride(), v.stride()
+    kp = vp = (0, 0, 0)
+    if k_scales is not None:
+        kp = (k_scales.data_ptr(), k_scales.stride(0), k_scales.stride(1))
+        vp = (v_scales.data_ptr(), v_scales.stride(0), v_scales.stride(1))
+    _C.run_tree_decode(_C.TREE_PARAMS.pack(
+        _C.dtype_code(q), code, _C.FLAG_FORCE_GENERIC if force_generic else 0, b, H, KVH, T, L, D, num_splits,
+        D ** -0.5 if sm_scale is None else sm_scale, len_ptr, tm_ptr, tm_sb, tm_st, q.data_ptr(), qs[0], qs[1], qs[2],
+        k.data_ptr(), ks[0], ks[1], ks[2], v.data_ptr(), vs[0], vs[1], vs[2], *kp, *vp, out.data_ptr(), H * T * D, D),
+        q.device, check_status)
+    return out
+
+
+def group_query_attention_tree(query, key, value, tree_mask=None, *, sm_scale=None, kv_lens=None, num_splits=0,
+                               force_generic=False, check_status=None):
+    """Attention of a tree of drafted tokens over a dense cache (the verification step of speculative decoding).
+
+    query (bsz, num_heads, T, head_dim); key / value (bsz, num_kv_heads, kv_len, head_dim), head_dim <= 256, any strides
+    with a contiguous last dim.  Sequence b uses its first kv_lens[b] rows (int32 (bsz,), default all); the last T of
+    them are the drafted tokens' own, already written: token u in row kv_lens[b] - T + u.  Token t sees every row before
+    those, and drafted token u where tree_mask[t, u] (bool, (T, T) or (bsz, T, T); default: u <= t, a chain).  What a
+    token does not see does not reach it, NaN and infinities included; a token that sees nothing gives zeros.
+    Logits are multiplied by sm_scale (default 1 / sqrt(head_dim)).  Returns (bsz, num_heads, T, head_dim)."""
+    _C.require_cuda(query, key, value)
+    if query.dim() != 4 or key.dim() != 4 or key.shape != value.shape:
+        raise ValueError("query (bsz, num_heads, T, head_dim) and key / value (bsz, num_kv_heads, kv_len, head_dim) expected; "
+                         f"got {tuple(query.shape)}, {tuple(key.shape)} and {tuple(value.shape)}")
+    if key.shape[0] != query.shape[0] or key.shape[3] != query.shape[3]:
+        raise ValueError(f"batch or head_dim mismatch between query {tuple(query.shape)} and key {tuple(key.shape)}")
+    if key.dtype != query.dtype or value.dtype != query.dtype:
+        raise ValueError("all tensors of one call must share a dtype")
+    k, v = (t if t.stride(3) == 1 or t.shape[3] == 1 else t.contiguous() for t in (key, value))
+    return _tree_decode(query, k, v, None, None, _C.CACHE_DENSE, tree_mask, sm_scale, kv_lens, num_splits, force_generic,
+                        check_status)
+
+
+def group_query_attention_quantized(query, cache, tree_mask=None, *, sm_scale=None, kv_lens=None, num_splits=0,
+                                    force_generic=False, check_status=None):
+    """Decode attention over an 8-bit cache (a QuantizedCache), read as it is held: the codes are widened in registers
+    and the scales applied to logits and probabilities.  query (bsz, num_heads, T, head_dim), T = 1 for a plain decode
+    step, float32, bfloat16 or float16.  kv_lens, tree_mask and sm_scale as in group_query_attention_tree (kv_lens
+    defaults to the cache's capacity).  Returns (bsz, num_heads, T, head_dim)."""
+    b, KVH, cap, D, code = quant_cache.check_cache(cache)
+    _C.require_cuda(cache.key_codes, query)
+    if query.dim() != 4 or query.shape[0] != b or query.shape[3] != D:
+        raise ValueError(f"query must be ({b}, num_heads, T, {D}); got {tuple(query.shape)}")
+    return _tree_decode(query, cache.key_codes, cache.value_codes, cache.key_scales, cache.value_scales, code, tree_mask,
+                        sm_scale, kv_lens, num_splits, force_generic, check_status)
 
 
 def xkv_group_decode(queries, key_A, key_Bs, value, value_Bs=None, *, theta, sm_scale=None,

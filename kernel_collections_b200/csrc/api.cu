@@ -321,4 +321,37 @@ int xkv_latent_append(const void* x, int64_t x_sb, const void* proj, int64_t p_s
                               in_dim, rank, capacity, static_cast<cudaStream_t>(stream));
 }
 
+size_t xkv_rotary_params_size(void) { return sizeof(xkv_rotary_params); }
+
+int xkv_rotary(const xkv_rotary_params* p, void* stream) {
+  if (!p || p->dtype < XKV_F32 || p->dtype > XKV_F16) return XKV_ERR_BAD_ARG;
+  if (p->batch <= 0 || p->num_heads <= 0 || p->num_kv_heads < 0 || p->num_tokens <= 0 || p->head_dim <= 0)
+    return XKV_ERR_BAD_ARG;
+  if (p->rotary_dim <= 0 || (p->rotary_dim & 1) || p->rotary_dim > p->head_dim) return XKV_ERR_BAD_ARG;
+  if (!p->q || !p->q_out || !p->inv_freq) return XKV_ERR_BAD_ARG;
+  if ((p->k != nullptr) != (p->num_kv_heads > 0) || (p->k != nullptr) != (p->k_out != nullptr)) return XKV_ERR_BAD_ARG;
+  return launch_rotary(*p, static_cast<cudaStream_t>(stream));
+}
+
+size_t xkv_cache_params_size(void) { return sizeof(xkv_cache_params); }
+
+static int cache_check(const xkv_cache_params* p) {
+  if (!p || p->dtype < XKV_F32 || p->dtype > XKV_F16) return XKV_ERR_BAD_ARG;
+  if (p->cache_code != XKV_CACHE_INT8 && p->cache_code != XKV_CACHE_E4M3) return XKV_ERR_BAD_ARG;
+  if (p->batch <= 0 || p->num_kv_heads <= 0 || p->num_tokens <= 0 || p->capacity <= 0 || p->head_dim <= 0)
+    return XKV_ERR_BAD_ARG;
+  if (!p->k || !p->v || !p->k_codes || !p->v_codes || !p->k_scales || !p->v_scales) return XKV_ERR_BAD_ARG;
+  return p->head_dim > 1024 ? XKV_ERR_UNSUPPORTED : XKV_OK;
+}
+
+int xkv_cache_append(const xkv_cache_params* p, void* stream) {
+  const int rc = cache_check(p);
+  return rc != XKV_OK ? rc : launch_cache(*p, true, static_cast<cudaStream_t>(stream));
+}
+
+int xkv_cache_read(const xkv_cache_params* p, void* stream) {
+  const int rc = cache_check(p);
+  return rc != XKV_OK ? rc : launch_cache(*p, false, static_cast<cudaStream_t>(stream));
+}
+
 }  // extern "C"

@@ -47,6 +47,10 @@ int launch_latent_append(const void* x, int64_t x_sb, const void* proj, int64_t 
                          int64_t l_sb, int64_t l_sl, const int32_t* positions, int position, int dtype, int batch,
                          int in_dim, int rank, int capacity, cudaStream_t st);
 
+// ---- rotary positions (rotary.cu) and the 8-bit cache (quant_cache.cu) --------------------------
+int launch_rotary(const xkv_rotary_params& p, cudaStream_t st);
+int launch_cache(const xkv_cache_params& p, bool write, cudaStream_t st);   // write: append, else read back
+
 // ---- tcgen05 key-reconstruction path (recon_tc_sm100.cu) ------------------------------------
 struct ReconTcPlan {
   int pair;             // CTA pairs (cta_group::2) instead of single CTAs
