@@ -43,11 +43,17 @@ __device__ __forceinline__ bool sees(const xkv_tree_params& p, int b, int t, int
 
 // ---- host side -------------------------------------------------------------------------------------------------
 struct TreePlan {
+  enum Kernel { kPortable, kStream } kernel;
   const char* name;
   int rows, splits;
   size_t off_o, off_ml, total_bytes;
 };
 void tree_layout(const xkv_tree_params& p, TreePlan* pl);      // fills the offsets from rows and splits
 int tree_merge(const tree::Args& a, cudaStream_t st);
+
+// few query rows on mma.sync (tree_stream_sm100.cu): head_dim 64 or 128, 16-byte aligned rows
+bool tree_stream_supported(const xkv_tree_params& p);
+void tree_stream_plan(const xkv_tree_params& p, TreePlan* pl);     // pl->rows set
+int tree_stream_decode(const tree::Args& a, cudaStream_t st);
 
 }  // namespace xkv

@@ -210,6 +210,7 @@ __global__ void __launch_bounds__(128) merge_kernel(const Args a) {
   const int part = warp % WARPS;
   const int64_t all = (int64_t)p.batch * p.num_kv_heads * a.rows;
   const bool live = row < all;
+  asm volatile("griddepcontrol.wait;" ::: "memory");      // the splits' results
   const float2* ml = a.part_ml + (live ? row : 0) * a.splits;
   float M = -CUDART_INF_F;
   for (int s = lane; s < a.splits; s += 32) M = fmaxf(M, ml[s].x);
@@ -267,9 +268,19 @@ int merge(const Args& a, cudaStream_t st) {
   const int64_t rows = (int64_t)a.p.batch * a.p.num_kv_heads * a.rows;
   const int64_t grid = a.splits >= 4 ? rows : (rows + 3) / 4;
   if (grid > 0x7fffffff) return XKV_ERR_UNSUPPORTED;
-  if (a.splits >= 4) merge_kernel<T, 4><<<(unsigned)grid, 128, 0, st>>>(a);
-  else merge_kernel<T, 1><<<(unsigned)grid, 128, 0, st>>>(a);
-  return cudaGetLastError() == cudaSuccess ? XKV_OK : XKV_ERR_LAUNCH;
+  // launched early: its blocks wait on the device for the kernel before it, not on the stream
+  cudaLaunchAttribute early;
+  early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  early.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)grid);
+  cfg.blockDim = dim3(128);
+  cfg.stream = st;
+  cfg.attrs = &early;
+  cfg.numAttrs = 1;
+  const cudaError_t e = a.splits >= 4 ? cudaLaunchKernelEx(&cfg, merge_kernel<T, 4>, a) : cudaLaunchKernelEx(&cfg, merge_kernel<T, 1>, a);
+  if (e != cudaSuccess) cudaGetLastError();
+  return e == cudaSuccess ? XKV_OK : XKV_ERR_LAUNCH;
 }
 
 int validate(const xkv_tree_params* p) {
@@ -283,10 +294,12 @@ int validate(const xkv_tree_params* p) {
   if (p->cache_code != XKV_CACHE_DENSE && (!p->k_scales || !p->v_scales)) return XKV_ERR_BAD_ARG;
   if (p->head_dim > 256) return XKV_ERR_UNSUPPORTED;
   if ((int64_t)p->batch * p->num_heads * p->num_tokens > 0x7fffffff) return XKV_ERR_UNSUPPORTED;
+  if (p->kv_len > 0x7fffffff - 4096) return XKV_ERR_UNSUPPORTED;      // token indices past the last tile stay 32-bit
   return XKV_OK;
 }
 
 void portable_plan(const xkv_tree_params& p, TreePlan* pl) {
+  pl->kernel = TreePlan::kPortable;
   pl->name = "portable";
   const int64_t ctas = (int64_t)p.batch * p.num_kv_heads * ceil_div(pl->rows, RB);
   const int tiles = ceil_div(p.kv_len, TT);
@@ -299,7 +312,8 @@ void portable_plan(const xkv_tree_params& p, TreePlan* pl) {
 
 bool make_plan(const xkv_tree_params& p, TreePlan* pl) {
   pl->rows = p.num_heads / p.num_kv_heads * p.num_tokens;
-  portable_plan(p, pl);
+  if (!(p.flags & XKV_FLAG_FORCE_GENERIC) && tree_stream_supported(p)) tree_stream_plan(p, pl);
+  else portable_plan(p, pl);
   if (p.num_splits > 0) pl->splits = p.num_splits < 64 ? p.num_splits : 64;
   tree_layout(p, pl);
   return true;
@@ -362,6 +376,7 @@ int xkv_tree_decode(const xkv_tree_params* p, void* ws, size_t ws_bytes, void* s
   a.part_o = reinterpret_cast<float*>(w + pl.off_o);
   a.part_ml = reinterpret_cast<float2*>(w + pl.off_ml);
   a.status = reinterpret_cast<int*>(w);
+  if (pl.kernel == TreePlan::kStream) return tree_stream_decode(a, st);
   int e;
   switch (p->dtype) {
     case XKV_F32: e = tree::portable<float>(a, st); break;
