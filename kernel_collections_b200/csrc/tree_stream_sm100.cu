@@ -32,21 +32,40 @@ template <> __device__ __forceinline__ float to_float<float>(float v) { return v
 template <typename T> __device__ __forceinline__ T from_float(float v) { return TypeTraits<T>::from_f(v); }
 template <> __device__ __forceinline__ float from_float<float>(float v) { return v; }
 
-__device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool live) {
+__device__ __forceinline__ void cp16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp16_or_zero(uint32_t dst, const void* src, bool live) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(live ? 16 : 0) : "memory");
 }
 __device__ __forceinline__ void cp4(uint32_t dst, const void* src, bool live) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(live ? 4 : 0) : "memory");
 }
-__device__ __forceinline__ uint4 lds128(uint32_t a) {
-  uint4 v;
-  asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a) : "memory");
-  return v;
+// 2^x, relative error below 2^-22; 0 for -inf
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
 }
-__device__ __forceinline__ float lds32f(uint32_t a) {
-  float v;
-  asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(a) : "memory");
-  return v;
+// two fp32 operations in one instruction
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  float2 r;
+  asm("{.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmul.rn.f32x2 z, x, y;\n\tmov.b64 {%0, %1}, z;}"
+      : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return r;
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 r;
+  asm("{.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmov.b64 z, {%6, %7};\n\tfma.rn.f32x2 z, x, y, z;\n\t"
+      "mov.b64 {%0, %1}, z;}"
+      : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return r;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 r;
+  asm("{.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tadd.rn.f32x2 z, x, y;\n\tmov.b64 {%0, %1}, z;}"
+      : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return r;
 }
 
 // Two halves from the bytes `sel` picks of x: int8 codes (sign bits flipped beforehand), e4m3 codes.
@@ -96,393 +115,434 @@ __global__ void __launch_bounds__(NT, 2) stream_kernel(const Args a) {
   extern __shared__ __align__(128) uint8_t smem[];
   const xkv_tree_params& p = a.p;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  const int blocks = (a.rows + RB - 1) / RB;
-  int id = blockIdx.x;
-  const int rb = id % blocks; id /= blocks;
-  const int split = id % a.splits; id /= a.splits;
-  const int h = id % p.num_kv_heads, b = id / p.num_kv_heads;
-  const Span sp = span_of(p, b);
-  const int units = (sp.len + S::UNIT - 1) / S::UNIT;
-  const int begin = (int)((int64_t)split * units / a.splits), end = (int)((int64_t)(split + 1) * units / a.splits);
   asm volatile("griddepcontrol.launch_dependents;");
   if (blockIdx.x == 0 && threadIdx.x < 8) a.status[threadIdx.x] = 0;       // nothing here waits: the status is always good
+  Walk walk = walk_of(a, lane);
+  Piece pc;
+  while (next_piece(a, walk, pc)) {
+    const int b = pc.b, h = pc.h, rb = pc.rb;
+    const Span sp = span_of(p, b);
+    const int begin = pc.begin, end = pc.end;
 
-  const uint32_t ring = smem_u32(smem) + warp * (STAGES * S::STAGE);
-  const uint8_t* kbase = static_cast<const uint8_t*>(p.k) + ((int64_t)b * p.k_sb + (int64_t)h * p.k_sh) * S::ES;
-  const uint8_t* vbase = static_cast<const uint8_t*>(p.v) + ((int64_t)b * p.v_sb + (int64_t)h * p.v_sh) * S::ES;
-  const float* ksc = Q8 ? p.k_scales + (int64_t)b * p.ks_sb + (int64_t)h * p.ks_sh : nullptr;
-  const float* vsc = Q8 ? p.v_scales + (int64_t)b * p.vs_sb + (int64_t)h * p.vs_sh : nullptr;
-  auto fetch = [&](int u, int stage) {        // this warp's tokens of unit u; rows past the length arrive as zeros
-    if (u < end) {
-      const int t0 = u * S::UNIT + warp * TOK;
-      const uint32_t dst = ring + stage * S::STAGE;
-      constexpr int RPI = 32 / S::CH;         // rows per iteration of the warp (CH <= 16)
+    uint8_t* const ring = smem + warp * (STAGES * S::STAGE);
+    const uint32_t ring_a = smem_u32(ring);
+    const uint8_t* kbase = static_cast<const uint8_t*>(p.k) + ((int64_t)b * p.k_sb + (int64_t)h * p.k_sh) * S::ES;
+    const uint8_t* vbase = static_cast<const uint8_t*>(p.v) + ((int64_t)b * p.v_sb + (int64_t)h * p.v_sh) * S::ES;
+    const float* ksc = Q8 ? p.k_scales + (int64_t)b * p.ks_sb + (int64_t)h * p.ks_sh : nullptr;
+    const float* vsc = Q8 ? p.v_scales + (int64_t)b * p.vs_sb + (int64_t)h * p.vs_sh : nullptr;
+    const int64_t k_pitch = p.k_sl * S::ES, v_pitch = p.v_sl * S::ES;
+    auto fetch = [&](int u, int stage) {        // this warp's tokens of unit u; rows past the length arrive as zeros
+      if (u < end) {
+        const int t0 = u * S::UNIT + warp * TOK;
+        const uint32_t dst = ring_a + stage * S::STAGE;
+        constexpr int RPI = 32 / S::CH;         // rows per iteration of the warp (CH <= 16)
+        const int r0 = lane / S::CH, c = lane % S::CH;
+        if (t0 + TOK <= sp.len) {
+          const uint8_t* ks = kbase + (int64_t)(t0 + r0) * k_pitch + c * 16;
+          const uint8_t* vs = vbase + (int64_t)(t0 + r0) * v_pitch + c * 16;
 #pragma unroll
-      for (int i = 0; i < TOK / RPI; ++i) {
-        const int row = i * RPI + lane / S::CH, c = lane % S::CH;
-        const bool live = t0 + row < sp.len;
-        const int64_t at = live ? t0 + row : 0;
-        cp16(dst + S::at(row, c), kbase + at * p.k_sl * S::ES + c * 16, live);
-        cp16(dst + HALF + S::at(row, c), vbase + at * p.v_sl * S::ES + c * 16, live);
-      }
-      if (Q8) {
-#pragma unroll
-        for (int i = 0; i < TOK; i += 32) {
-          const int row = i + lane;
-          const bool live = t0 + row < sp.len;
-          cp4(dst + 2 * HALF + row * 4, ksc + (live ? t0 + row : 0), live);
-          cp4(dst + 2 * HALF + TOK * 4 + row * 4, vsc + (live ? t0 + row : 0), live);
-        }
-      }
-    }
-    asm volatile("cp.async.commit_group;" ::: "memory");
-  };
-#pragma unroll
-  for (int i = 0; i < STAGES - 1; ++i) fetch(begin + i, i);
-
-  // ---- queries: rows of this block as fp32 in shared memory, then as MMA fragments in registers --------------
-  float* qs = reinterpret_cast<float*>(smem + NW * STAGES * S::STAGE);
-  const int T_ = p.num_tokens, G = p.num_heads / p.num_kv_heads;
-  for (int r = warp; r < RB; r += NW) {
-    const int row = rb * RB + r;
-    const T* q = static_cast<const T*>(p.q) + (int64_t)b * p.q_sb + (int64_t)(h * G + row / T_) * p.q_sh + (int64_t)(row % T_) * p.q_st;
-    for (int d = lane; d < D; d += 32) qs[r * S::QS + d] = row < a.rows ? to_float(q[d]) : 0.f;
-  }
-  __syncthreads();
-  float row_scale[2];                       // score = accumulator * row_scale (* key scale)
-  uint32_t qf[TERMS][KS][4];
-#pragma unroll
-  for (int r = 0; r < 2; ++r) {
-    const float* q = qs + (g + r * 8) * S::QS;
-    float up = 1.f;
-    row_scale[r] = a.scale_log2;
-    if (Q8) {
-      float top = 0.f;
-      for (int d = t; d < D; d += 4) top = fmaxf(top, fabsf(q[d]));
-      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-      if (top > 0.f && top < CUDART_INF_F) {
-        const int e = min(max(14 - (int)(((__float_as_uint(top) >> 23) & 255u)) + 127, -120), 120);
-        up = __uint_as_float((uint32_t)(e + 127) << 23);
-        row_scale[r] = a.scale_log2 * __uint_as_float((uint32_t)(127 - e) << 23);
-      }
-    }
-#pragma unroll
-    for (int s = 0; s < KS; ++s)
-#pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        const int d = S::dim0(s, t) + 2 * k;
-        const float x = q[d] * up, y = q[d + 1] * up;
-        const uint32_t hi = TypeTraits<M>::pack2(x, y);
-        qf[0][s][r + 2 * k] = hi;
-        if (TERMS == 2) {
-          const float2 f = TypeTraits<M>::unpack2(hi);
-          qf[TERMS - 1][s][r + 2 * k] = TypeTraits<M>::pack2(x - f.x, y - f.y);
-        }
-      }
-  }
-
-  float ref[2] = {-CUDART_INF_F, -CUDART_INF_F}, l[2] = {0.f, 0.f};     // rows g and g + 8
-  float unit_v[2] = {0.f, 0.f};                                         // power of two the value scales are relative to
-  float o[NO][4];
-#pragma unroll
-  for (int n = 0; n < NO; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
-
-  int stage = 0;
-  for (int u = begin; u < end; ++u) {
-    const int nxt = stage + STAGES - 1;
-    fetch(u + STAGES - 1, nxt >= STAGES ? nxt - STAGES : nxt);
-    asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 1) : "memory");
-    __syncwarp();
-    const int t0 = u * S::UNIT + warp * TOK;
-    const uint32_t sk = ring + stage * S::STAGE, sv = sk + HALF, ss = sv + HALF;
-    if (++stage == STAGES) stage = 0;
-    if (t0 >= sp.len) continue;
-    const bool plain = t0 + TOK <= sp.first;     // every row sees every token of this step
-
-    // ---- scores ---------------------------------------------------------------------------------------------
-    float sc[NS][4];
-#pragma unroll
-    for (int n = 0; n < NS; ++n) {
-      sc[n][0] = sc[n][1] = sc[n][2] = sc[n][3] = 0.f;
-#pragma unroll
-      for (int i = 0; i < S::CH / 4; ++i) {
-        uint4 w4 = lds128(sk + S::at(n * 8 + g, S::piece(i, t)));
-        uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
-#pragma unroll
-        for (int k = 0; k < S::KPC; ++k) {
-          const int s = i * S::KPC + k;
-          uint32_t b0, b1;
-          if (Q8) {
-            if (CODE == XKV_CACHE_INT8) w[k] ^= 0x80808080u;
-            b0 = widen<CODE>(w[k], 0);
-            b1 = widen<CODE>(w[k], 1);
-          } else {
-            b0 = w[(2 * k) & 3];
-            b1 = w[(2 * k + 1) & 3];
+          for (int i = 0; i < TOK / RPI; ++i) {
+            const uint32_t at = dst + S::at(i * RPI + r0, c);
+            cp16(at, ks);
+            cp16(at + HALF, vs);
+            ks += RPI * k_pitch;
+            vs += RPI * v_pitch;
           }
-          TypeTraits<M>::mma(sc[n], qf[0][s], b0, b1);
-          if (TERMS == 2) TypeTraits<M>::mma(sc[n], qf[TERMS - 1][s], b0, b1);
-        }
-      }
-    }
-    // ---- scale, hide, maximum -----------------------------------------------------------------------------------
-    // sc becomes the score in the log2 domain; vs the value scales of this thread's tokens
-    float vs[NS][2];
-    uint32_t vis[2] = {0xffffffffu, 0xffffffffu};        // bit 2n + e: row sees token 8n + 2t + e
-    float mx[2] = {-CUDART_INF_F, -CUDART_INF_F};
+          if (Q8) {
 #pragma unroll
-    for (int n = 0; n < NS; ++n)
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const int tok = n * 8 + 2 * t + e;
-        float k = 1.f;
-        if (Q8) {
-          k = lds32f(ss + tok * 4);
-          vs[n][e] = lds32f(ss + TOK * 4 + tok * 4);
-        }
-#pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          float x = sc[n][2 * r + e] * row_scale[r];
-          if (Q8) x *= k;
-          if (!plain) {
-            const int row = min(rb * RB + g + r * 8, a.rows - 1);
-            if (t0 + tok >= sp.len || !sees(p, b, row % T_, t0 + tok, sp.first)) {
-              vis[r] &= ~(1u << (2 * n + e));
-              x = -CUDART_INF_F;
+            for (int i = 0; i < TOK; i += 32) {
+              cp4(dst + 2 * HALF + (i + lane) * 4, ksc + t0 + i + lane, true);
+              cp4(dst + 2 * HALF + TOK * 4 + (i + lane) * 4, vsc + t0 + i + lane, true);
             }
           }
-          sc[n][2 * r + e] = x;
-          mx[r] = fmaxf(mx[r], x);
+        } else {
+          for (int i = 0; i < TOK / RPI; ++i) {
+            const int row = i * RPI + r0;
+            const bool live = t0 + row < sp.len;
+            const int64_t at = live ? t0 + row : 0;
+            cp16_or_zero(dst + S::at(row, c), kbase + at * k_pitch + c * 16, live);
+            cp16_or_zero(dst + HALF + S::at(row, c), vbase + at * v_pitch + c * 16, live);
+          }
+          if (Q8) {
+            for (int i = 0; i < TOK; i += 32) {
+              const int row = i + lane;
+              const bool live = t0 + row < sp.len;
+              cp4(dst + 2 * HALF + row * 4, ksc + (live ? t0 + row : 0), live);
+              cp4(dst + 2 * HALF + TOK * 4 + row * 4, vsc + (live ? t0 + row : 0), live);
+            }
+          }
         }
       }
-    bool move = false;
+      asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+#pragma unroll
+    for (int i = 0; i < STAGES - 1; ++i) fetch(begin + i, i);
+
+    // ---- queries: rows of this block as fp32 in shared memory, then as MMA fragments in registers --------------
+    float* qs = reinterpret_cast<float*>(smem + NW * STAGES * S::STAGE);
+    const int T_ = p.num_tokens, G = p.num_heads / p.num_kv_heads;
+    for (int r = warp; r < RB; r += NW) {
+      const int row = rb * RB + r;
+      const T* q = static_cast<const T*>(p.q) + (int64_t)b * p.q_sb + (int64_t)(h * G + row / T_) * p.q_sh + (int64_t)(row % T_) * p.q_st;
+      for (int d = lane; d < D; d += 32) qs[r * S::QS + d] = row < a.rows ? to_float(q[d]) : 0.f;
+    }
+    __syncthreads();
+    float row_scale[2];                       // score = accumulator * row_scale (* key scale); positive
+    uint32_t qf[TERMS][KS][4];
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
-      mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 1));
-      mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 2));
-      move |= mx[r] > ref[r] + SLACK;
-    }
-    // the value scales' common power of two: above the largest finite one that a row sees
-    float top[2] = {0.f, 0.f};
-    if (Q8) {
-#pragma unroll
-      for (int n = 0; n < NS; ++n)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const float v = fabsf(vs[n][e]);
-          const float f = v < CUDART_INF_F ? v : 0.f;
-#pragma unroll
-          for (int r = 0; r < 2; ++r)
-            if (plain ? r == 0 : (vis[r] >> (2 * n + e) & 1)) top[r] = fmaxf(top[r], f);
+      const float* q = qs + (g + r * 8) * S::QS;
+      // the sign of the scale goes to the queries, so that the largest product is the largest score; a scale of zero too
+      float up = a.scale_log2 < 0.f ? -1.f : 1.f;
+      row_scale[r] = fmaxf(fabsf(a.scale_log2), 1.17549435e-38f);
+      if (a.scale_log2 == 0.f) {
+        up = 0.f;
+        row_scale[r] = 1.f;
+      } else if (Q8) {
+        float top = 0.f;
+        for (int d = t; d < D; d += 4) top = fmaxf(top, fabsf(q[d]));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        if (top > 0.f && top < CUDART_INF_F) {
+          const int e = min(max(14 - (int)(((__float_as_uint(top) >> 23) & 255u)) + 127, -120), 120);
+          up *= __uint_as_float((uint32_t)(e + 127) << 23);
+          row_scale[r] = fmaxf(row_scale[r] * __uint_as_float((uint32_t)(127 - e) << 23), 1.17549435e-38f);
         }
-#pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        if (r == 1 && plain) { top[1] = top[0]; break; }
-        top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 1));
-        top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 2));
       }
-      move |= top[0] > unit_v[0] || top[1] > unit_v[1];
-    }
-    if (__any_sync(0xffffffffu, move)) {
 #pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        const float to = mx[r] > ref[r] + SLACK ? mx[r] : ref[r];      // by the row's own scores: rows stay independent
-        const float alpha = to == -CUDART_INF_F ? 1.f : exp2f(ref[r] - to);
-        ref[r] = to;
-        l[r] *= alpha;
-        float f = alpha;
-        if (Q8 && top[r] > unit_v[r]) {
-          // a power of two up to twice the largest scale (capped at 2^127); both are powers of two: the ratio is exact
-          const uint32_t e = min((__float_as_uint(top[r]) >> 23) + 1u, 254u);
-          const float to_v = __uint_as_float(e << 23);
-          f *= unit_v[r] / to_v;
-          unit_v[r] = to_v;
+      for (int s = 0; s < KS; ++s)
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          const int d = S::dim0(s, t) + 2 * k;
+          const float x = q[d] * up, y = q[d + 1] * up;
+          const uint32_t hi = TypeTraits<M>::pack2(x, y);
+          qf[0][s][r + 2 * k] = hi;
+          if (TERMS == 2) {
+            const float2 f = TypeTraits<M>::unpack2(hi);
+            qf[TERMS - 1][s][r + 2 * k] = TypeTraits<M>::pack2(x - f.x, y - f.y);
+          }
         }
-#pragma unroll
-        for (int n = 0; n < NO; ++n) { o[n][2 * r] *= f; o[n][2 * r + 1] *= f; }
-      }
     }
-    // ---- weights --------------------------------------------------------------------------------------------------
-    uint32_t pf[TERMS][NS][2];             // [n][r]: tokens 8n + 2t, + 1 of row g + 8r
+
+    float ref[2] = {-CUDART_INF_F, -CUDART_INF_F};                        // rows g and g + 8
+    float2 l[2] = {{0.f, 0.f}, {0.f, 0.f}};
+    float unit_v[2] = {0.f, 0.f};                                         // power of two the value scales are relative to
+    float o[NO][4];
 #pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      const float base = ref[r] == -CUDART_INF_F ? 0.f : ref[r] - LIFT;
-      const float inv = Q8 ? (unit_v[r] > 0.f ? 1.f / unit_v[r] : 0.f) : 1.f;
+    for (int n = 0; n < NO; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
+
+    int stage = 0;
+    for (int u = begin; u < end; ++u) {
+      const int nxt = stage + STAGES - 1;
+      fetch(u + STAGES - 1, nxt >= STAGES ? nxt - STAGES : nxt);
+      asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 1) : "memory");
+      __syncwarp();
+      const int t0 = u * S::UNIT + warp * TOK;
+      const uint8_t* const sk = ring + stage * S::STAGE;
+      const uint8_t* const sv = sk + HALF;
+      const float* const kss = reinterpret_cast<const float*>(sv + HALF);      // key scales, then value scales
+      if (++stage == STAGES) stage = 0;
+      if (t0 >= sp.len) continue;
+      const bool plain = t0 + TOK <= sp.first;     // every row sees every token of this step
+
+      // ---- scores ---------------------------------------------------------------------------------------------
+      float sc[NS][4];
 #pragma unroll
       for (int n = 0; n < NS; ++n) {
-        float w0 = exp2f(sc[n][2 * r] - base), w1 = exp2f(sc[n][2 * r + 1] - base);
-        if (Q8) {
-          l[r] += w0 + w1;
-          // a hidden token's scale may be anything
-          w0 = plain || (vis[r] >> (2 * n) & 1) ? w0 * (vs[n][0] * inv) : 0.f;
-          w1 = plain || (vis[r] >> (2 * n + 1) & 1) ? w1 * (vs[n][1] * inv) : 0.f;
-        }
-        const uint32_t hi = TypeTraits<M>::pack2(w0, w1);
-        pf[0][n][r] = hi;
-        const float2 f = TypeTraits<M>::unpack2(hi);
-        if (TERMS == 2) pf[TERMS - 1][n][r] = TypeTraits<M>::pack2(w0 - f.x, w1 - f.y);
-        if (!Q8) l[r] += f.x + f.y;         // the sum of what P.V multiplies with: the rounding cancels in O / l
-      }
-    }
-    // Drafted rows may be hidden from some query rows only, and 0 * NaN is NaN: elements that are not finite are taken
-    // out of the value tile here and added after the product, to the rows that see their token.
-    uint64_t bad = 0;
-    if (!plain && CODE != XKV_CACHE_INT8) {
-      for (int i = lane; i < TOK * S::CH; i += 32) {
-        const int row = i / S::CH;
-        const uint32_t ad = sv + S::at(row, i % S::CH);
-        const uint4 v4 = lds128(ad);
-        uint32_t v[4] = {v4.x, v4.y, v4.z, v4.w};
-        bool hit = false;
+        sc[n][0] = sc[n][1] = sc[n][2] = sc[n][3] = 0.f;
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          if (Q8) {
+        for (int i = 0; i < S::CH / 4; ++i) {
+          const uint4 w4 = *reinterpret_cast<const uint4*>(sk + S::at(n * 8 + g, S::piece(i, t)));
+          uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
 #pragma unroll
-            for (int e = 0; e < 32; e += 8)
-              if ((v[k] >> e & 0x7fu) == 0x7fu) { v[k] &= ~(0xffu << e); hit = true; }
-          } else {
-            constexpr uint32_t EXP = std::is_same<M, __half>::value ? 0x7c00u : 0x7f80u;
-#pragma unroll
-            for (int e = 0; e < 32; e += 16)
-              if ((v[k] >> e & EXP) == EXP) { v[k] &= ~(0xffffu << e); hit = true; }
+          for (int k = 0; k < S::KPC; ++k) {
+            const int s = i * S::KPC + k;
+            uint32_t b0, b1;
+            if (Q8) {
+              if (CODE == XKV_CACHE_INT8) w[k] ^= 0x80808080u;
+              b0 = widen<CODE>(w[k], 0);
+              b1 = widen<CODE>(w[k], 1);
+            } else {
+              b0 = w[(2 * k) & 3];
+              b1 = w[(2 * k + 1) & 3];
+            }
+            TypeTraits<M>::mma(sc[n], qf[0][s], b0, b1);
+            if (TERMS == 2) TypeTraits<M>::mma(sc[n], qf[TERMS - 1][s], b0, b1);
           }
         }
-        if (hit) {
-          bad |= 1ull << row;
-          asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(ad), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]) : "memory");
-        }
       }
-      const uint32_t lo = __reduce_or_sync(0xffffffffu, (uint32_t)bad), hi = __reduce_or_sync(0xffffffffu, (uint32_t)(bad >> 32));
-      bad = (uint64_t)hi << 32 | lo;
-      __syncwarp();
-    }
-    // ---- O += P.V ----------------------------------------------------------------------------------------------------
-#pragma unroll
-    for (int kk = 0; kk < TOK / 16; ++kk) {
-      uint32_t af[TERMS][4];
-#pragma unroll
-      for (int x = 0; x < TERMS; ++x) {
-        af[x][0] = pf[x][2 * kk][0]; af[x][1] = pf[x][2 * kk][1];
-        af[x][2] = pf[x][2 * kk + 1][0]; af[x][3] = pf[x][2 * kk + 1][1];
-      }
+      // ---- key scales, hidden tokens, maximum (scores still without row_scale) ----------------------------------------
+      uint32_t vis[2] = {0xffffffffu, 0xffffffffu};        // bit 2n + e: row sees token 8n + 2t + e
       if (Q8) {
-        constexpr int WORDS = D / 32;           // words of four dims per token that a thread widens
-        uint32_t w[4][WORDS];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int row = kk * 16 + (j >> 1) * 8 + 2 * t + (j & 1);
-          if (WORDS == 4) {
-            const uint4 v = lds128(sv + S::at(row, g));
-            w[j][0] = v.x; w[j][1 % WORDS] = v.y; w[j][2 % WORDS] = v.z; w[j][3 % WORDS] = v.w;
-          } else {
-            uint32_t x, y;
-            asm volatile("ld.shared.v2.b32 {%0,%1}, [%2];" : "=r"(x), "=r"(y) : "r"(sv + S::at(row, g >> 1) + (g & 1) * 8) : "memory");
-            w[j][0] = x; w[j][1 % WORDS] = y;
+        for (int n = 0; n < NS; ++n) {
+          const float2 k = *reinterpret_cast<const float2*>(kss + n * 8 + 2 * t);
+#pragma unroll
+          for (int r = 0; r < 2; ++r) {
+            const float2 x = mul2(make_float2(sc[n][2 * r], sc[n][2 * r + 1]), k);
+            sc[n][2 * r] = x.x;
+            sc[n][2 * r + 1] = x.y;
           }
-          if (CODE == XKV_CACHE_INT8)
-#pragma unroll
-            for (int i = 0; i < WORDS; ++i) w[j][i] ^= 0x80808080u;
         }
+      }
+      if (!plain) {
 #pragma unroll
-        for (int i = 0; i < WORDS; ++i)
+        for (int r = 0; r < 2; ++r) {
+          const int tok = min(rb * RB + g + r * 8, a.rows - 1) % T_;
 #pragma unroll
-          for (int k = 0; k < 2; ++k) {        // dims 4i + 2k, + 1: bytes of two tokens side by side
-            const uint32_t x = __byte_perm(w[0][i], w[1][i], k ? 0x7362u : 0x5140u);
-            const uint32_t y = __byte_perm(w[2][i], w[3][i], k ? 0x7362u : 0x5140u);
+          for (int n = 0; n < NS; ++n)
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-              const int n = 4 * i + 2 * k + e;
-              const uint32_t b0 = widen<CODE>(x, e), b1 = widen<CODE>(y, e);
-              TypeTraits<M>::mma(o[n], af[0], b0, b1);
-              if (TERMS == 2) TypeTraits<M>::mma(o[n], af[TERMS - 1], b0, b1);
+              const int at = t0 + n * 8 + 2 * t + e;
+              if (at >= sp.len || !sees(p, b, tok, at, sp.first)) {
+                vis[r] &= ~(1u << (2 * n + e));
+                sc[n][2 * r + e] = -CUDART_INF_F;
+              }
             }
-          }
-      } else {
-        const int mi = lane >> 3, r = lane & 7;
-        const int row = kk * 16 + (mi & 1) * 8 + r;
-#pragma unroll
-        for (int n = 0; n < NO; n += 2) {
-          uint32_t v[4];
-          asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
-                       : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3])
-                       : "r"(sv + S::at(row, n + (mi >> 1))) : "memory");
-          TypeTraits<M>::mma(o[n], af[0], v[0], v[1]);
-          TypeTraits<M>::mma(o[n + 1], af[0], v[2], v[3]);
         }
       }
-    }
-    // column of accumulator n, element e: 8-bit caches deal 16 (8) consecutive dims to the eight column groups
-    while (bad) {
-      const int tok = __ffsll((long long)bad) - 1;
-      bad &= bad - 1;
-      const uint8_t* vr = vbase + (int64_t)(t0 + tok) * p.v_sl * S::ES;
+      float mx[2] = {-CUDART_INF_F, -CUDART_INF_F};
+      bool move = false;
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
-        const int row = rb * RB + g + r * 8;
-        if (row >= a.rows || !sees(p, b, row % T_, t0 + tok, sp.first)) continue;
 #pragma unroll
-        for (int n = 0; n < NO; ++n)
+        for (int n = 0; n < NS; ++n) mx[r] = fmaxf(mx[r], fmaxf(sc[n][2 * r], sc[n][2 * r + 1]));
+        mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 1));
+        mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 2)) * row_scale[r];
+        move |= mx[r] > ref[r] + SLACK;
+      }
+      // the value scales' common power of two: above the largest finite one that a row sees
+      float top[2] = {0.f, 0.f};
+      if (Q8 && plain) {
+        uint32_t m = 0;
 #pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const int d = Q8 ? (2 * t + e) * NO + n : n * 8 + 2 * t + e;
-            const float x = Q8 ? __half2float(__half(__nv_cvt_fp8_to_halfraw(vr[d], __NV_E4M3)))
-                               : to_float(reinterpret_cast<const M*>(vr)[d]);
-            if (!(fabsf(x) < CUDART_INF_F)) o[n][2 * r + e] += x;
+        for (int i = 0; i < TOK; i += 32) {
+          const uint32_t v = __float_as_uint(kss[TOK + i + lane]) & 0x7fffffffu;     // magnitudes order as integers
+          m = max(m, v < 0x7f800000u ? v : 0u);
+        }
+        top[0] = top[1] = __uint_as_float(__reduce_max_sync(0xffffffffu, m));
+      } else if (Q8) {
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+#pragma unroll
+          for (int n = 0; n < NS; ++n)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const float v = fabsf(kss[TOK + n * 8 + 2 * t + e]);
+              if (v < CUDART_INF_F && (vis[r] >> (2 * n + e) & 1)) top[r] = fmaxf(top[r], v);
+            }
+          top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 1));
+          top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 2));
+        }
+      }
+      if (Q8) move |= top[0] > unit_v[0] || top[1] > unit_v[1];
+      if (__any_sync(0xffffffffu, move)) {
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          const float to = mx[r] > ref[r] + SLACK ? mx[r] : ref[r];      // by the row's own scores: rows stay independent
+          const float alpha = to == -CUDART_INF_F ? 1.f : exp2f(ref[r] - to);
+          ref[r] = to;
+          l[r].x *= alpha;
+          l[r].y *= alpha;
+          float f = alpha;
+          if (Q8 && top[r] > unit_v[r]) {
+            // a power of two up to twice the largest scale (capped at 2^127); both are powers of two: the ratio is exact
+            const uint32_t e = min((__float_as_uint(top[r]) >> 23) + 1u, 254u);
+            const float to_v = __uint_as_float(e << 23);
+            f *= unit_v[r] / to_v;
+            unit_v[r] = to_v;
           }
+#pragma unroll
+          for (int n = 0; n < NO; ++n) { o[n][2 * r] *= f; o[n][2 * r + 1] *= f; }
+        }
+      }
+      // ---- weights --------------------------------------------------------------------------------------------------
+      uint32_t pf[TERMS][NS][2];             // [n][r]: tokens 8n + 2t, + 1 of row g + 8r
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        const float base = ref[r] == -CUDART_INF_F ? 0.f : LIFT - ref[r];
+        const float inv = Q8 ? (unit_v[r] > 0.f ? 1.f / unit_v[r] : 0.f) : 1.f;
+#pragma unroll
+        for (int n = 0; n < NS; ++n) {
+          const float2 x = fma2(make_float2(sc[n][2 * r], sc[n][2 * r + 1]), make_float2(row_scale[r], row_scale[r]), make_float2(base, base));
+          float2 w = make_float2(ex2(x.x), ex2(x.y));
+          if (Q8) {
+            l[r] = add2(l[r], w);
+            const float2 v = *reinterpret_cast<const float2*>(kss + TOK + n * 8 + 2 * t);
+            w = mul2(w, mul2(v, make_float2(inv, inv)));
+            if (!plain) {                    // a hidden token's scale may be anything
+              if (!(vis[r] >> (2 * n) & 1)) w.x = 0.f;
+              if (!(vis[r] >> (2 * n + 1) & 1)) w.y = 0.f;
+            }
+          }
+          const uint32_t hi = TypeTraits<M>::pack2(w.x, w.y);
+          pf[0][n][r] = hi;
+          if (TERMS == 2) {
+            const float2 f = TypeTraits<M>::unpack2(hi);
+            pf[TERMS - 1][n][r] = TypeTraits<M>::pack2(w.x - f.x, w.y - f.y);
+          }
+          if (!Q8) l[r] = add2(l[r], TypeTraits<M>::unpack2(hi));   // the sum of what P.V multiplies with: the rounding cancels
+        }
+      }
+      // Drafted rows may be hidden from some query rows only, and 0 * NaN is NaN: elements that are not finite are taken
+      // out of the value tile here and added after the product, to the rows that see their token.
+      uint64_t bad = 0;
+      if (!plain && CODE != XKV_CACHE_INT8) {
+        for (int i = lane; i < TOK * S::CH; i += 32) {
+          const int row = i / S::CH;
+          uint4* ad = reinterpret_cast<uint4*>(const_cast<uint8_t*>(sv) + S::at(row, i % S::CH));
+          const uint4 v4 = *ad;
+          uint32_t v[4] = {v4.x, v4.y, v4.z, v4.w};
+          bool hit = false;
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            if (Q8) {
+#pragma unroll
+              for (int e = 0; e < 32; e += 8)
+                if ((v[k] >> e & 0x7fu) == 0x7fu) { v[k] &= ~(0xffu << e); hit = true; }
+            } else {
+              constexpr uint32_t EXP = std::is_same<M, __half>::value ? 0x7c00u : 0x7f80u;
+#pragma unroll
+              for (int e = 0; e < 32; e += 16)
+                if ((v[k] >> e & EXP) == EXP) { v[k] &= ~(0xffffu << e); hit = true; }
+            }
+          }
+          if (hit) {
+            bad |= 1ull << row;
+            *ad = make_uint4(v[0], v[1], v[2], v[3]);
+          }
+        }
+        const uint32_t lo = __reduce_or_sync(0xffffffffu, (uint32_t)bad), hi = __reduce_or_sync(0xffffffffu, (uint32_t)(bad >> 32));
+        bad = (uint64_t)hi << 32 | lo;
+        __syncwarp();
+      }
+      // ---- O += P.V ----------------------------------------------------------------------------------------------------
+#pragma unroll
+      for (int kk = 0; kk < TOK / 16; ++kk) {
+        uint32_t af[TERMS][4];
+#pragma unroll
+        for (int x = 0; x < TERMS; ++x) {
+          af[x][0] = pf[x][2 * kk][0]; af[x][1] = pf[x][2 * kk][1];
+          af[x][2] = pf[x][2 * kk + 1][0]; af[x][3] = pf[x][2 * kk + 1][1];
+        }
+        if (Q8) {
+          constexpr int WORDS = D / 32;           // words of four dims per token that a thread widens
+          uint32_t w[4][WORDS];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const int row = kk * 16 + (j >> 1) * 8 + 2 * t + (j & 1);
+            if (WORDS == 4) {
+              const uint4 v = *reinterpret_cast<const uint4*>(sv + S::at(row, g));
+              w[j][0] = v.x; w[j][1 % WORDS] = v.y; w[j][2 % WORDS] = v.z; w[j][3 % WORDS] = v.w;
+            } else {
+              const uint2 v = *reinterpret_cast<const uint2*>(sv + S::at(row, g >> 1) + (g & 1) * 8);
+              w[j][0] = v.x; w[j][1 % WORDS] = v.y;
+            }
+            if (CODE == XKV_CACHE_INT8)
+#pragma unroll
+              for (int i = 0; i < WORDS; ++i) w[j][i] ^= 0x80808080u;
+          }
+#pragma unroll
+          for (int i = 0; i < WORDS; ++i)
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {        // dims 4i + 2k, + 1: bytes of two tokens side by side
+              const uint32_t x = __byte_perm(w[0][i], w[1][i], k ? 0x7362u : 0x5140u);
+              const uint32_t y = __byte_perm(w[2][i], w[3][i], k ? 0x7362u : 0x5140u);
+#pragma unroll
+              for (int e = 0; e < 2; ++e) {
+                const int n = 4 * i + 2 * k + e;
+                const uint32_t b0 = widen<CODE>(x, e), b1 = widen<CODE>(y, e);
+                TypeTraits<M>::mma(o[n], af[0], b0, b1);
+                if (TERMS == 2) TypeTraits<M>::mma(o[n], af[TERMS - 1], b0, b1);
+              }
+            }
+        } else {
+          const int mi = lane >> 3, r = lane & 7;
+          const int row = kk * 16 + (mi & 1) * 8 + r;
+#pragma unroll
+          for (int n = 0; n < NO; n += 2) {
+            uint32_t v[4];
+            asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+                         : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3])
+                         : "r"(smem_u32(sv) + S::at(row, n + (mi >> 1))) : "memory");
+            TypeTraits<M>::mma(o[n], af[0], v[0], v[1]);
+            TypeTraits<M>::mma(o[n + 1], af[0], v[2], v[3]);
+          }
+        }
+      }
+      // column of accumulator n, element e: 8-bit caches deal 16 (8) consecutive dims to the eight column groups
+      while (bad) {
+        const int tok = __ffsll((long long)bad) - 1;
+        bad &= bad - 1;
+        const uint8_t* vr = vbase + (int64_t)(t0 + tok) * p.v_sl * S::ES;
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          const int row = rb * RB + g + r * 8;
+          if (row >= a.rows || !sees(p, b, row % T_, t0 + tok, sp.first)) continue;
+#pragma unroll
+          for (int n = 0; n < NO; ++n)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const int d = Q8 ? (2 * t + e) * NO + n : n * 8 + 2 * t + e;
+              const float x = Q8 ? __half2float(__half(__nv_cvt_fp8_to_halfraw(vr[d], __NV_E4M3)))
+                                 : to_float(reinterpret_cast<const M*>(vr)[d]);
+              if (!(fabsf(x) < CUDART_INF_F)) o[n][2 * r + e] += x;
+            }
+        }
+      }
+      __syncwarp();       // every lane is done with the stage before the next copies into it
+    }
+
+    // ---- join the four warps ------------------------------------------------------------------------------------------
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    __syncthreads();
+    constexpr int OS = D + 4;
+    float* acc = reinterpret_cast<float*>(smem);               // [warp][row][OS]
+    float2* ml = reinterpret_cast<float2*>(qs);                // [warp][row]
+    static_assert(NW * RB * OS * 4 <= NW * STAGES * S::STAGE, "the ring holds the partial outputs");
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      float sum = l[r].x + l[r].y;
+      sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+      sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+      float* row = acc + (warp * RB + g + r * 8) * OS;
+      const float f = Q8 ? unit_v[r] : 1.f;
+#pragma unroll
+      for (int n = 0; n < NO; ++n)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) row[Q8 ? (2 * t + e) * NO + n : n * 8 + 2 * t + e] = o[n][2 * r + e] * f;
+      if (t == 0) ml[warp * RB + g + r * 8] = make_float2(ref[r] == -CUDART_INF_F ? ref[r] : ref[r] - LIFT, sum);
+    }
+    __syncthreads();
+    const int live = min(RB, a.rows - rb * RB);
+    for (int i = threadIdx.x; i < live * (D / 4); i += NT) {
+      const int r = i / (D / 4), d = (i - r * (D / 4)) * 4;
+      float m = -CUDART_INF_F;
+#pragma unroll
+      for (int w = 0; w < NW; ++w) m = fmaxf(m, ml[w * RB + r].x);
+      const float use = m == -CUDART_INF_F ? 0.f : m;
+      float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+      float sum = 0.f;
+#pragma unroll
+      for (int w = 0; w < NW; ++w) {
+        const float2 e = ml[w * RB + r];
+        const float f = exp2f(e.x - use);
+        const float4 y = *reinterpret_cast<const float4*>(acc + (w * RB + r) * OS + d);
+        x.x = fmaf(f, y.x, x.x); x.y = fmaf(f, y.y, x.y); x.z = fmaf(f, y.z, x.z); x.w = fmaf(f, y.w, x.w);
+        sum = fmaf(f, e.y, sum);
+      }
+      if (pc.whole) {
+        const float inv = sum == 0.f ? 0.f : 1.f / sum;
+        const int64_t out_row = (int64_t)h * a.rows + rb * RB + r;
+        T* out = static_cast<T*>(p.out) + (int64_t)b * p.o_sb + out_row * p.o_sr + d;
+        out[0] = from_float<T>(x.x * inv); out[1] = from_float<T>(x.y * inv);
+        out[2] = from_float<T>(x.z * inv); out[3] = from_float<T>(x.w * inv);
+      } else {
+        *reinterpret_cast<float4*>(a.part_o + (pc.id * RB + r) * D + d) = x;
+        if (d == 0) a.part_ml[pc.id * RB + r] = make_float2(m, sum);
       }
     }
-    __syncwarp();       // every lane is done with the stage before the next copies into it
-  }
-
-  // ---- join the four warps ------------------------------------------------------------------------------------------
-  asm volatile("cp.async.wait_all;" ::: "memory");
-  __syncthreads();
-  constexpr int OS = D + 4;
-  float* acc = reinterpret_cast<float*>(smem);               // [warp][row][OS]
-  float2* ml = reinterpret_cast<float2*>(qs);                // [warp][row]
-  static_assert(NW * RB * OS * 4 <= NW * STAGES * S::STAGE, "the ring holds the partial outputs");
-#pragma unroll
-  for (int r = 0; r < 2; ++r) {
-    l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
-    l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
-    float* row = acc + (warp * RB + g + r * 8) * OS;
-    const float f = Q8 ? unit_v[r] : 1.f;
-#pragma unroll
-    for (int n = 0; n < NO; ++n)
-#pragma unroll
-      for (int e = 0; e < 2; ++e) row[Q8 ? (2 * t + e) * NO + n : n * 8 + 2 * t + e] = o[n][2 * r + e] * f;
-    if (t == 0) ml[warp * RB + g + r * 8] = make_float2(ref[r] == -CUDART_INF_F ? ref[r] : ref[r] - LIFT, l[r]);
-  }
-  __syncthreads();
-  const int64_t row0 = (int64_t)(b * p.num_kv_heads + h) * a.rows + rb * RB;
-  const int live = min(RB, a.rows - rb * RB);
-  for (int i = threadIdx.x; i < live * (D / 4); i += NT) {
-    const int r = i / (D / 4), d = (i - r * (D / 4)) * 4;
-    float m = -CUDART_INF_F;
-#pragma unroll
-    for (int w = 0; w < NW; ++w) m = fmaxf(m, ml[w * RB + r].x);
-    const float use = m == -CUDART_INF_F ? 0.f : m;
-    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-    float sum = 0.f;
-#pragma unroll
-    for (int w = 0; w < NW; ++w) {
-      const float2 e = ml[w * RB + r];
-      const float f = exp2f(e.x - use);
-      const float4 y = *reinterpret_cast<const float4*>(acc + (w * RB + r) * OS + d);
-      x.x = fmaf(f, y.x, x.x); x.y = fmaf(f, y.y, x.y); x.z = fmaf(f, y.z, x.z); x.w = fmaf(f, y.w, x.w);
-      sum = fmaf(f, e.y, sum);
-    }
-    if (a.splits == 1) {
-      const float inv = sum == 0.f ? 0.f : 1.f / sum;
-      const int64_t out_row = (int64_t)h * a.rows + rb * RB + r;
-      T* out = static_cast<T*>(p.out) + (int64_t)b * p.o_sb + out_row * p.o_sr + d;
-      out[0] = from_float<T>(x.x * inv); out[1] = from_float<T>(x.y * inv);
-      out[2] = from_float<T>(x.z * inv); out[3] = from_float<T>(x.w * inv);
-    } else {
-      *reinterpret_cast<float4*>(a.part_o + ((row0 + r) * a.splits + split) * D + d) = x;
-      if (d == 0) a.part_ml[(row0 + r) * a.splits + split] = make_float2(m, sum);
-    }
+    __syncthreads();       // the ring is free for the next piece
   }
 }
 
@@ -494,9 +554,7 @@ int launch(const Args& a, cudaStream_t st) {
     cudaGetLastError();
     return XKV_ERR_LAUNCH;
   }
-  const int64_t grid = (int64_t)a.splits * ceil_div(a.rows, RB) * a.p.num_kv_heads * a.p.batch;
-  if (grid > 0x7fffffff) return XKV_ERR_UNSUPPORTED;
-  kern<<<(unsigned)grid, NT, smem, st>>>(a);
+  kern<<<(unsigned)a.grid, NT, smem, st>>>(a);
   return cudaGetLastError() == cudaSuccess ? XKV_OK : XKV_ERR_LAUNCH;
 }
 template <typename T, int CODE, int TERMS>
@@ -530,30 +588,18 @@ bool tree_stream_supported(const xkv_tree_params& p) {
 void tree_stream_plan(const xkv_tree_params& p, TreePlan* pl) {
   pl->kernel = TreePlan::kStream;
   pl->name = "stream";
-  const int es = p.cache_code == XKV_CACHE_DENSE ? 2 : 1;
-  const int unit = tree::NW * tree::HALF / (p.head_dim * es);
-  const int units = ceil_div(p.kv_len, unit);
-  const int64_t slots = 2 * device_sm_count();            // two blocks per SM
-  const int64_t rows = (int64_t)p.batch * p.num_kv_heads * ceil_div(pl->rows, tree::RB);
-  // as few splits as fill the SMs evenly; a block costs about two units to start, join and merge
-  int best = 1;
-  int64_t best_cost = -1;
-  for (int s = 1; s <= units && s <= 128; ++s) {
-    const int64_t cost = (rows * s + slots - 1) / slots * (ceil_div(units, s) + 2);
-    if (best_cost < 0 || cost < best_cost) { best_cost = cost; best = s; }
-  }
-  pl->splits = best;
+  pl->block_rows = tree::RB;
+  pl->unit_tokens = tree::NW * tree::HALF / (p.head_dim * (p.cache_code == XKV_CACHE_DENSE ? 2 : 1));
+  pl->slots = 2 * device_sm_count();            // two blocks per SM
 }
 
 int tree_stream_decode(const tree::Args& a, cudaStream_t st) {
   using namespace tree;
-  int rc;
   if (a.p.cache_code == XKV_CACHE_DENSE)
-    rc = a.p.dtype == XKV_BF16 ? by_dim<__nv_bfloat16, XKV_CACHE_DENSE, 1>(a, st) : by_dim<__half, XKV_CACHE_DENSE, 1>(a, st);
-  else if (a.p.dtype == XKV_BF16) rc = by_code<__nv_bfloat16, 1>(a, st);
-  else if (a.p.dtype == XKV_F16) rc = by_code<__half, 1>(a, st);
-  else rc = by_code<float, 2>(a, st);
-  return rc != XKV_OK || a.splits == 1 ? rc : tree_merge(a, st);
+    return a.p.dtype == XKV_BF16 ? by_dim<__nv_bfloat16, XKV_CACHE_DENSE, 1>(a, st) : by_dim<__half, XKV_CACHE_DENSE, 1>(a, st);
+  if (a.p.dtype == XKV_BF16) return by_code<__nv_bfloat16, 1>(a, st);
+  if (a.p.dtype == XKV_F16) return by_code<__half, 1>(a, st);
+  return by_code<float, 2>(a, st);
 }
 
 }  // namespace xkv
