@@ -2,14 +2,20 @@
 //
 // Up to 16 query rows (heads of a KV head x drafted tokens) share one pass, so the arithmetic is far below the tensor
 // rate and the pass is bound by HBM as long as the instructions per cache byte stay low.  Hence:
-//  * Every warp is on its own: it copies its 4 KB of K and of V (32 tokens of 128 codes, 16 of 128 halves) into a
-//    private three-stage ring with cp.async and meets the other warps only at the end.  No block barrier, nothing to wait
-//    for but its own copies.
+//  * Every warp is on its own: it copies its 4 KB of K and of V (32 tokens of 128 codes, 16 of 128 halves) into a private
+//    two-stage ring with cp.async and meets the other warps only at the end of a piece.  No block barrier in the loop,
+//    nothing to wait for but its own copies.
+//  * With at most 8 query rows the tokens (and, for P.V, the dims) are the 16 rows of the MMA and the queries its 8 columns:
+//    half the MMAs, accumulators and exponentials of the 16-row form, which pads the queries to 16.  The weights then
+//    turn from accumulator to operand layout by movmatrix.
 //  * 8-bit codes are widened in registers on their way into the MMA and never written back.  The contraction index of
 //    Q.K^T may be permuted freely, so a thread takes 16 consecutive codes of a token (one 16-byte read) and Q is laid
 //    out to match.  For P.V the two tokens of an operand register are interleaved by byte permutes.  int8: the code
 //    with its sign bit flipped under the exponent byte 0x64 is the half 1024 + 128 + code; e4m3 converts in pairs.
 //    Widened codes are exact in fp16 (8 significant bits), so the products run in fp16 whatever the query type.
+//  * The 1152 above the int8 keys is not subtracted from every element: the score's accumulator starts at -1152 sum(q).
+//    The partial sums are 1152 |sum q| large, an fp32 rounding of which is below 2^-17 of sum |q||code|.  (fp32
+//    queries subtract it; so do the values, whose sums run over thousands of tokens.)
 //  * Scales never touch the codes: the key scale multiplies the score, the value scale the weight.
 //  * fp16 ranges: a query row is multiplied by a power of two that brings its largest element to 2^14..2^15, and divided
 //    out of the scores in fp32: elements below 2^-28 of the largest lose bits, others none.  Weights carry the factor 2^12
@@ -25,7 +31,7 @@ namespace tree {
 using namespace sm100;
 namespace {
 
-constexpr int NW = 4, NT = NW * 32, RB = 16, STAGES = 3, HALF = 4096;   // HALF: bytes of K (or V) per warp and stage
+constexpr int NW = 4, NT = NW * 32, STAGES = 2, HALF = 4096;   // HALF: bytes of K (or V) per warp and stage
 
 template <typename T> __device__ __forceinline__ float to_float(T v) { return TypeTraits<T>::to_f(v); }
 template <> __device__ __forceinline__ float to_float<float>(float v) { return v; }
@@ -80,6 +86,14 @@ __device__ __forceinline__ uint32_t widen_e4m3(uint32_t x, int high) {
   asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"(two));
   return r;
 }
+// int8 codes still 1152 above their value (sign bits flipped beforehand)
+__device__ __forceinline__ uint32_t raise_int8(uint32_t x, int high) { return __byte_perm(x, 0x64646464u, high ? 0x4342u : 0x4140u); }
+// 8 x 8 transpose of 16-bit elements across the warp
+__device__ __forceinline__ uint32_t transpose8(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
 // bytes 0, 1 of x (high = 0) or 2, 3 as two halves
 template <int CODE> __device__ __forceinline__ uint32_t widen(uint32_t x, int high) {
   return CODE == XKV_CACHE_INT8 ? widen_int8(x, high ? 0x4342u : 0x4140u) : widen_e4m3(x, high);
@@ -94,8 +108,8 @@ struct Shape {
   static constexpr int UNIT = NW * TOK;            // tokens per block and stage
   static constexpr int SCALES = ES == 1 ? TOK * 8 : 0;
   static constexpr int STAGE = 2 * HALF + SCALES;
-  static constexpr int QS = D + 4;                 // row stride of the staged queries (floats)
-  static constexpr int SMEM = NW * STAGES * STAGE + RB * QS * 4;
+  static constexpr int FRAGS = D / 16 * 512;       // bytes of one term of the queries as MMA operands
+  static_assert(16 * D * 4 <= STAGE, "the second stage of the first warp holds the staged queries");
   // pieces of a row are permuted by the row so that the reads below touch every bank once
   static __device__ __forceinline__ int at(int row, int c) { return row * ROWB + ((c ^ (CH >= 8 ? row & 7 : (row >> 1) & 3)) << 4); }
   // piece i (of CH / 4) that lane t of a quad reads of its token, and the first of the four dims of k-step s
@@ -104,12 +118,20 @@ struct Shape {
   static __device__ __forceinline__ int dim0(int s, int t) { return piece(s / KPC, t) * (16 / ES) + (s % KPC) * 4; }
 };
 
-template <typename T, int CODE, int D, int TERMS>
-__global__ void __launch_bounds__(NT, 2) stream_kernel(const Args a) {
+// Blocks per SM.
+template <int TERMS> constexpr int resident() { return TERMS == 1 ? 3 : 2; }
+
+// RB query rows per strip.  A thread's two rows and its tokens of every 8: RB == 16: rows g, g + 8 and tokens 2t, 2t + 1;
+// RB == 8: rows 2t, 2t + 1 and token g.
+template <typename T, int CODE, int D, int TERMS, int RB>
+__global__ void __launch_bounds__(NT, resident<TERMS>()) stream_kernel(const Args a) {
   using S = Shape<T, CODE, D>;
-  constexpr bool Q8 = CODE != XKV_CACHE_DENSE;
+  constexpr bool Q8 = CODE != XKV_CACHE_DENSE, WIDE = RB == 16;
+  constexpr bool RAISED = CODE == XKV_CACHE_INT8 && TERMS == 1;       // keys enter the product 1152 above their value
   using M = typename std::conditional<Q8, __half, typename std::conditional<std::is_same<T, float>::value, __half, T>::type>::type;
   constexpr int TOK = S::TOK, NS = TOK / 8, KS = D / 16, NO = D / 8;
+  constexpr int E = WIDE ? 2 : 1;                  // tokens of every 8 that a thread scores, for each of its rows
+  constexpr int QV = WIDE ? 1 : 2;                 // k-steps per 16 bytes of query operand
   // weights are 2^(score - reference + LIFT); the reference follows the maximum when it is passed by more than SLACK
   constexpr float LIFT = std::is_same<M, __half>::value ? 12.f : 0.f, SLACK = std::is_same<M, __half>::value ? 3.f : 8.f;
   extern __shared__ __align__(128) uint8_t smem[];
@@ -175,61 +197,98 @@ __global__ void __launch_bounds__(NT, 2) stream_kernel(const Args a) {
       }
       asm volatile("cp.async.commit_group;" ::: "memory");
     };
-#pragma unroll
-    for (int i = 0; i < STAGES - 1; ++i) fetch(begin + i, i);
+    fetch(begin, 0);
 
-    // ---- queries: rows of this block as fp32 in shared memory, then as MMA fragments in registers --------------
-    float* qs = reinterpret_cast<float*>(smem + NW * STAGES * S::STAGE);
+    // ---- queries: scaled rows as fp32 in the free second stage, then as MMA operands --------------------------------
+    float* qs = reinterpret_cast<float*>(smem + S::STAGE);                         // [row][D]
+    uint4* qfrag = reinterpret_cast<uint4*>(smem + NW * STAGES * S::STAGE);        // [term][k-step / QV][lane]
+    float2* qrow = reinterpret_cast<float2*>(qfrag + TERMS * S::FRAGS / 16);       // [row]: row_scale, start of the score
     const int T_ = p.num_tokens, G = p.num_heads / p.num_kv_heads;
     for (int r = warp; r < RB; r += NW) {
       const int row = rb * RB + r;
       const T* q = static_cast<const T*>(p.q) + (int64_t)b * p.q_sb + (int64_t)(h * G + row / T_) * p.q_sh + (int64_t)(row % T_) * p.q_st;
-      for (int d = lane; d < D; d += 32) qs[r * S::QS + d] = row < a.rows ? to_float(q[d]) : 0.f;
-    }
-    __syncthreads();
-    float row_scale[2];                       // score = accumulator * row_scale (* key scale); positive
-    uint32_t qf[TERMS][KS][4];
+      float x[D / 32], top = 0.f;
 #pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      const float* q = qs + (g + r * 8) * S::QS;
+      for (int i = 0; i < D / 32; ++i) {
+        x[i] = row < a.rows ? to_float(q[i * 32 + lane]) : 0.f;
+        top = fmaxf(top, fabsf(x[i]));
+      }
+      top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top)));
       // the sign of the scale goes to the queries, so that the largest product is the largest score; a scale of zero too
-      float up = a.scale_log2 < 0.f ? -1.f : 1.f;
-      row_scale[r] = fmaxf(fabsf(a.scale_log2), 1.17549435e-38f);
+      float up = a.scale_log2 < 0.f ? -1.f : 1.f, scale = fmaxf(fabsf(a.scale_log2), 1.17549435e-38f);
       if (a.scale_log2 == 0.f) {
         up = 0.f;
-        row_scale[r] = 1.f;
-      } else if (Q8) {
-        float top = 0.f;
-        for (int d = t; d < D; d += 4) top = fmaxf(top, fabsf(q[d]));
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        if (top > 0.f && top < CUDART_INF_F) {
-          const int e = min(max(14 - (int)(((__float_as_uint(top) >> 23) & 255u)) + 127, -120), 120);
-          up *= __uint_as_float((uint32_t)(e + 127) << 23);
-          row_scale[r] = fmaxf(row_scale[r] * __uint_as_float((uint32_t)(127 - e) << 23), 1.17549435e-38f);
-        }
+        scale = 1.f;
+      } else if (Q8 && top > 0.f && top < CUDART_INF_F) {
+        const int e = min(max(14 - (int)(((__float_as_uint(top) >> 23) & 255u)) + 127, -120), 120);
+        up *= __uint_as_float((uint32_t)(e + 127) << 23);
+        scale = fmaxf(scale * __uint_as_float((uint32_t)(127 - e) << 23), 1.17549435e-38f);
       }
+      float sum = 0.f;
 #pragma unroll
-      for (int s = 0; s < KS; ++s)
+      for (int i = 0; i < D / 32; ++i) {
+        x[i] *= up;
+        if (RAISED) sum += __half2float(__float2half_rn(x[i]));       // of what the product multiplies with
+        qs[r * D + i * 32 + lane] = x[i];
+      }
+      if (RAISED)
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          const int d = S::dim0(s, t) + 2 * k;
-          const float x = q[d] * up, y = q[d + 1] * up;
-          const uint32_t hi = TypeTraits<M>::pack2(x, y);
-          qf[0][s][r + 2 * k] = hi;
+        for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      if (lane == 0) qrow[r] = make_float2(scale, RAISED ? -1152.f * sum : 0.f);
+    }
+    __syncthreads();
+    for (int s = warp; s < KS; s += NW) {
+      uint32_t f[TERMS][2 * E];         // WIDE: (row g, dims 0 1), (g + 8, 0 1), (g, 2 3), (g + 8, 2 3); else (g, 0 1), (g, 2 3)
+#pragma unroll
+      for (int k = 0; k < 2; ++k)
+#pragma unroll
+        for (int r = 0; r < E; ++r) {
+          const float* q = qs + (g + r * 8) * D + S::dim0(s, t) + 2 * k;
+          f[0][r + E * k] = TypeTraits<M>::pack2(q[0], q[1]);
           if (TERMS == 2) {
-            const float2 f = TypeTraits<M>::unpack2(hi);
-            qf[TERMS - 1][s][r + 2 * k] = TypeTraits<M>::pack2(x - f.x, y - f.y);
+            const float2 z = TypeTraits<M>::unpack2(f[0][r + E * k]);
+            f[TERMS - 1][r + E * k] = TypeTraits<M>::pack2(q[0] - z.x, q[1] - z.y);
           }
         }
-    }
-
-    float ref[2] = {-CUDART_INF_F, -CUDART_INF_F};                        // rows g and g + 8
-    float2 l[2] = {{0.f, 0.f}, {0.f, 0.f}};
-    float unit_v[2] = {0.f, 0.f};                                         // power of two the value scales are relative to
-    float o[NO][4];
 #pragma unroll
-    for (int n = 0; n < NO; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
+      for (int x = 0; x < TERMS; ++x) {
+        if constexpr (WIDE) qfrag[(x * KS + s) * 32 + lane] = make_uint4(f[x][0], f[x][1], f[x][2], f[x][3]);
+        else reinterpret_cast<uint2*>(qfrag)[((x * KS + s) / 2 * 32 + lane) * 2 + (s & 1)] = make_uint2(f[x][0], f[x][1]);
+      }
+    }
+    float row_scale[2], start[2];       // score = accumulator * row_scale (* key scale), row_scale > 0
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      const float2 q = qrow[WIDE ? g + 8 * r : 2 * t + r];
+      row_scale[r] = q.x;
+      start[r] = q.y;
+    }
+    __syncthreads();
+
+    float ref[2] = {-CUDART_INF_F, -CUDART_INF_F};
+    float2 l[2] = {{0.f, 0.f}, {0.f, 0.f}};                               // WIDE: [row]{token}; else [0]{row}
+    float unit_v[2] = {0.f, 0.f};                                         // power of two the value scales are relative to
+    // WIDE: [n]: rows g, g + 8 x columns 2t, 2t + 1 of 8 dims n.  Else [n / 2]: columns g of dims n, n + 1 x rows 2t, 2t + 1
+    float o[NO * E / 2][4];
+#pragma unroll
+    for (int n = 0; n < NO * E / 2; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
+    // the largest over the lanes that share a thread's rows
+    auto across = [](float x) {
+      if (WIDE) {
+        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
+        return fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
+      }
+      x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
+      x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
+      return fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
+    };
+    const int tok0 = WIDE ? 2 * t : g;          // + 8n + e: this thread's tokens
+    // query row and dim of o[n][i]; 8-bit caches deal NO consecutive dims to each of the eight columns
+    auto row_of = [&](int i) { return WIDE ? g + 8 * (i >> 1) : 2 * t + (i & 1); };
+    auto dim_of = [&](int n, int i) {
+      const int col = WIDE ? 2 * t + (i & 1) : g, tile = WIDE ? n : 2 * n + (i >> 1);
+      return Q8 ? col * NO + tile : tile * 8 + col;
+    };
 
     int stage = 0;
     for (int u = begin; u < end; ++u) {
@@ -246,57 +305,85 @@ __global__ void __launch_bounds__(NT, 2) stream_kernel(const Args a) {
       const bool plain = t0 + TOK <= sp.first;     // every row sees every token of this step
 
       // ---- scores ---------------------------------------------------------------------------------------------
-      float sc[NS][4];
+      // WIDE: sc[n][2r + e], token 8n + 2t + e of row g + 8r; else sc[n / 2][2 (n & 1) + r], token 8n + g of row 2t + r
+      float sc[NS * E / 2][4];
 #pragma unroll
-      for (int n = 0; n < NS; ++n) {
-        sc[n][0] = sc[n][1] = sc[n][2] = sc[n][3] = 0.f;
+      for (int n = 0; n < NS * E / 2; ++n)
 #pragma unroll
-        for (int i = 0; i < S::CH / 4; ++i) {
-          const uint4 w4 = *reinterpret_cast<const uint4*>(sk + S::at(n * 8 + g, S::piece(i, t)));
-          uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
+        for (int i = 0; i < 4; ++i) sc[n][i] = start[WIDE ? i >> 1 : i & 1];
+#pragma unroll
+      for (int i = 0; i < S::CH / 4; ++i) {
+        uint4 qf[TERMS][S::KPC / QV];
+#pragma unroll
+        for (int x = 0; x < TERMS; ++x)
+#pragma unroll
+          for (int k = 0; k < S::KPC / QV; ++k) qf[x][k] = qfrag[(x * KS + i * S::KPC) / QV * 32 + k * 32 + lane];
+#pragma unroll
+        for (int n = 0; n < NS; n += 2 / E) {
+          uint32_t w[2 / E][4];
+#pragma unroll
+          for (int m = 0; m < 2 / E; ++m) {
+            const uint4 w4 = *reinterpret_cast<const uint4*>(sk + S::at((n + m) * 8 + g, S::piece(i, t)));
+            w[m][0] = w4.x; w[m][1] = w4.y; w[m][2] = w4.z; w[m][3] = w4.w;
+          }
 #pragma unroll
           for (int k = 0; k < S::KPC; ++k) {
-            const int s = i * S::KPC + k;
-            uint32_t b0, b1;
-            if (Q8) {
-              if (CODE == XKV_CACHE_INT8) w[k] ^= 0x80808080u;
-              b0 = widen<CODE>(w[k], 0);
-              b1 = widen<CODE>(w[k], 1);
-            } else {
-              b0 = w[(2 * k) & 3];
-              b1 = w[(2 * k + 1) & 3];
+            uint32_t f[2 / E][2];         // tokens of tile n + m, dims 0 1 and 2 3
+#pragma unroll
+            for (int m = 0; m < 2 / E; ++m) {
+              if (Q8) {
+                const uint32_t x = CODE == XKV_CACHE_INT8 ? w[m][k] ^ 0x80808080u : w[m][k];
+                f[m][0] = RAISED ? raise_int8(x, 0) : widen<CODE>(x, 0);
+                f[m][1] = RAISED ? raise_int8(x, 1) : widen<CODE>(x, 1);
+              } else {
+                f[m][0] = w[m][(2 * k) & 3];
+                f[m][1] = w[m][(2 * k + 1) & 3];
+              }
             }
-            TypeTraits<M>::mma(sc[n], qf[0][s], b0, b1);
-            if (TERMS == 2) TypeTraits<M>::mma(sc[n], qf[TERMS - 1][s], b0, b1);
+#pragma unroll
+            for (int x = 0; x < TERMS; ++x) {
+              const uint4 q = qf[x][k / QV];
+              if constexpr (WIDE) {
+                const uint32_t qa[4] = {q.x, q.y, q.z, q.w};
+                TypeTraits<M>::mma(sc[n], qa, f[0][0], f[0][1]);
+              } else {
+                const uint32_t ka[4] = {f[0][0], f[1][0], f[0][1], f[1][1]};
+                TypeTraits<M>::mma(sc[n / 2], ka, k & 1 ? q.z : q.x, k & 1 ? q.w : q.y);
+              }
+            }
           }
         }
       }
-      // ---- key scales, hidden tokens, maximum (scores still without row_scale) ----------------------------------------
-      uint32_t vis[2] = {0xffffffffu, 0xffffffffu};        // bit 2n + e: row sees token 8n + 2t + e
+      auto score = [&](int n, int r, int e) -> float& { return WIDE ? sc[n][2 * r + e] : sc[n / 2][2 * (n & 1) + r]; };
+      // ---- key scales, hidden tokens, maximum (scores still without row_scale) --------------------------------------
+      uint32_t vis[2] = {0xffffffffu, 0xffffffffu};        // bit E n + e: row sees token 8n + tok0 + e
       if (Q8) {
 #pragma unroll
         for (int n = 0; n < NS; ++n) {
-          const float2 k = *reinterpret_cast<const float2*>(kss + n * 8 + 2 * t);
+          float2 k;
+          if (WIDE) k = *reinterpret_cast<const float2*>(kss + n * 8 + tok0);
+          else k.x = k.y = kss[n * 8 + tok0];
 #pragma unroll
-          for (int r = 0; r < 2; ++r) {
-            const float2 x = mul2(make_float2(sc[n][2 * r], sc[n][2 * r + 1]), k);
-            sc[n][2 * r] = x.x;
-            sc[n][2 * r + 1] = x.y;
+          for (int r = 0; r < E; ++r) {
+            float* x = WIDE ? &sc[n][2 * r] : &sc[n / 2][2 * (n & 1)];
+            const float2 y = mul2(make_float2(x[0], x[1]), k);
+            x[0] = y.x;
+            x[1] = y.y;
           }
         }
       }
       if (!plain) {
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
-          const int tok = min(rb * RB + g + r * 8, a.rows - 1) % T_;
+          const int tok = min(rb * RB + (WIDE ? g + 8 * r : 2 * t + r), a.rows - 1) % T_;
 #pragma unroll
           for (int n = 0; n < NS; ++n)
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              const int at = t0 + n * 8 + 2 * t + e;
+            for (int e = 0; e < E; ++e) {
+              const int at = t0 + n * 8 + tok0 + e;
               if (at >= sp.len || !sees(p, b, tok, at, sp.first)) {
-                vis[r] &= ~(1u << (2 * n + e));
-                sc[n][2 * r + e] = -CUDART_INF_F;
+                vis[r] &= ~(1u << (E * n + e));
+                score(n, r, e) = -CUDART_INF_F;
               }
             }
         }
@@ -306,9 +393,10 @@ __global__ void __launch_bounds__(NT, 2) stream_kernel(const Args a) {
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
 #pragma unroll
-        for (int n = 0; n < NS; ++n) mx[r] = fmaxf(mx[r], fmaxf(sc[n][2 * r], sc[n][2 * r + 1]));
-        mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 1));
-        mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 2)) * row_scale[r];
+        for (int n = 0; n < NS; ++n)
+#pragma unroll
+          for (int e = 0; e < E; ++e) mx[r] = fmaxf(mx[r], score(n, r, e));
+        mx[r] = across(mx[r]) * row_scale[r];
         move |= mx[r] > ref[r] + SLACK;
       }
       // the value scales' common power of two: above the largest finite one that a row sees
@@ -327,62 +415,76 @@ __global__ void __launch_bounds__(NT, 2) stream_kernel(const Args a) {
 #pragma unroll
           for (int n = 0; n < NS; ++n)
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              const float v = fabsf(kss[TOK + n * 8 + 2 * t + e]);
-              if (v < CUDART_INF_F && (vis[r] >> (2 * n + e) & 1)) top[r] = fmaxf(top[r], v);
+            for (int e = 0; e < E; ++e) {
+              const float v = fabsf(kss[TOK + n * 8 + tok0 + e]);
+              if (v < CUDART_INF_F && (vis[r] >> (E * n + e) & 1)) top[r] = fmaxf(top[r], v);
             }
-          top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 1));
-          top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 2));
+          top[r] = across(top[r]);
         }
       }
       if (Q8) move |= top[0] > unit_v[0] || top[1] > unit_v[1];
       if (__any_sync(0xffffffffu, move)) {
+        float f[2];
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
           const float to = mx[r] > ref[r] + SLACK ? mx[r] : ref[r];      // by the row's own scores: rows stay independent
-          const float alpha = to == -CUDART_INF_F ? 1.f : exp2f(ref[r] - to);
+          f[r] = to == -CUDART_INF_F ? 1.f : exp2f(ref[r] - to);
           ref[r] = to;
-          l[r].x *= alpha;
-          l[r].y *= alpha;
-          float f = alpha;
+          if (WIDE) l[r] = mul2(l[r], make_float2(f[r], f[r]));
+          else if (r == 1) l[0] = mul2(l[0], make_float2(f[0], f[1]));
+        }
+#pragma unroll
+        for (int r = 0; r < 2; ++r)
           if (Q8 && top[r] > unit_v[r]) {
             // a power of two up to twice the largest scale (capped at 2^127); both are powers of two: the ratio is exact
             const uint32_t e = min((__float_as_uint(top[r]) >> 23) + 1u, 254u);
-            const float to_v = __uint_as_float(e << 23);
-            f *= unit_v[r] / to_v;
-            unit_v[r] = to_v;
+            const float to = __uint_as_float(e << 23);
+            f[r] *= unit_v[r] / to;
+            unit_v[r] = to;
           }
 #pragma unroll
-          for (int n = 0; n < NO; ++n) { o[n][2 * r] *= f; o[n][2 * r + 1] *= f; }
-        }
+        for (int n = 0; n < NO * E / 2; ++n)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) o[n][i] *= f[WIDE ? i >> 1 : i & 1];
       }
-      // ---- weights --------------------------------------------------------------------------------------------------
-      uint32_t pf[TERMS][NS][2];             // [n][r]: tokens 8n + 2t, + 1 of row g + 8r
+      // ---- weights ------------------------------------------------------------------------------------------------
+      // pf as operands of P.V: WIDE [term][n][r] tokens 8n + 2t, + 1 of row g + 8r; else [term][n][0] the same of row g
+      uint32_t pf[TERMS][NS][E];
+      {
+        float base[2], inv[2];
 #pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        const float base = ref[r] == -CUDART_INF_F ? 0.f : LIFT - ref[r];
-        const float inv = Q8 ? (unit_v[r] > 0.f ? 1.f / unit_v[r] : 0.f) : 1.f;
+        for (int r = 0; r < 2; ++r) {
+          base[r] = ref[r] == -CUDART_INF_F ? 0.f : LIFT - ref[r];
+          inv[r] = Q8 ? (unit_v[r] > 0.f ? 1.f / unit_v[r] : 0.f) : 1.f;
+        }
 #pragma unroll
-        for (int n = 0; n < NS; ++n) {
-          const float2 x = fma2(make_float2(sc[n][2 * r], sc[n][2 * r + 1]), make_float2(row_scale[r], row_scale[r]), make_float2(base, base));
-          float2 w = make_float2(ex2(x.x), ex2(x.y));
-          if (Q8) {
-            l[r] = add2(l[r], w);
-            const float2 v = *reinterpret_cast<const float2*>(kss + TOK + n * 8 + 2 * t);
-            w = mul2(w, mul2(v, make_float2(inv, inv)));
-            if (!plain) {                    // a hidden token's scale may be anything
-              if (!(vis[r] >> (2 * n) & 1)) w.x = 0.f;
-              if (!(vis[r] >> (2 * n + 1) & 1)) w.y = 0.f;
+        for (int n = 0; n < NS; ++n)
+#pragma unroll
+          for (int r = 0; r < E; ++r) {          // WIDE: a row's two tokens; else a token's two rows
+            const float* s2 = WIDE ? &sc[n][2 * r] : &sc[n / 2][2 * (n & 1)];
+            const float2 scale = WIDE ? make_float2(row_scale[r], row_scale[r]) : make_float2(row_scale[0], row_scale[1]);
+            const float2 x = fma2(make_float2(s2[0], s2[1]), scale, WIDE ? make_float2(base[r], base[r]) : make_float2(base[0], base[1]));
+            float2 w = make_float2(ex2(x.x), ex2(x.y));
+            if (Q8) {
+              l[r] = add2(l[r], w);
+              float2 v;
+              if (WIDE) v = *reinterpret_cast<const float2*>(kss + TOK + n * 8 + tok0);
+              else v.x = v.y = kss[TOK + n * 8 + tok0];
+              w = mul2(w, mul2(v, WIDE ? make_float2(inv[r], inv[r]) : make_float2(inv[0], inv[1])));
+              if (!plain) {                    // a hidden token's scale may be anything
+                if (!(vis[WIDE ? r : 0] >> (E * n) & 1)) w.x = 0.f;
+                if (!(vis[WIDE ? r : 1] >> (E * n + E - 1) & 1)) w.y = 0.f;
+              }
+            }
+            const uint32_t hi = TypeTraits<M>::pack2(w.x, w.y);
+            const float2 f = TypeTraits<M>::unpack2(hi);
+            if (!Q8) l[r] = add2(l[r], f);      // the sum of what P.V multiplies with: the rounding cancels
+            pf[0][n][r] = WIDE ? hi : transpose8(hi);
+            if (TERMS == 2) {
+              const uint32_t lo = TypeTraits<M>::pack2(w.x - f.x, w.y - f.y);
+              pf[TERMS - 1][n][r] = WIDE ? lo : transpose8(lo);
             }
           }
-          const uint32_t hi = TypeTraits<M>::pack2(w.x, w.y);
-          pf[0][n][r] = hi;
-          if (TERMS == 2) {
-            const float2 f = TypeTraits<M>::unpack2(hi);
-            pf[TERMS - 1][n][r] = TypeTraits<M>::pack2(w.x - f.x, w.y - f.y);
-          }
-          if (!Q8) l[r] = add2(l[r], TypeTraits<M>::unpack2(hi));   // the sum of what P.V multiplies with: the rounding cancels
-        }
       }
       // Drafted rows may be hidden from some query rows only, and 0 * NaN is NaN: elements that are not finite are taken
       // out of the value tile here and added after the product, to the rows that see their token.
@@ -416,27 +518,35 @@ __global__ void __launch_bounds__(NT, 2) stream_kernel(const Args a) {
         bad = (uint64_t)hi << 32 | lo;
         __syncwarp();
       }
-      // ---- O += P.V ----------------------------------------------------------------------------------------------------
+      // ---- O += P.V ------------------------------------------------------------------------------------------------
 #pragma unroll
       for (int kk = 0; kk < TOK / 16; ++kk) {
-        uint32_t af[TERMS][4];
+        // values of dims n (f[0], f[1]: tokens 2t, + 1 and 2t + 8, + 9 of column g) and n + 1 (f[2], f[3])
+        auto product = [&](int n, const uint32_t (&f)[4]) {
 #pragma unroll
-        for (int x = 0; x < TERMS; ++x) {
-          af[x][0] = pf[x][2 * kk][0]; af[x][1] = pf[x][2 * kk][1];
-          af[x][2] = pf[x][2 * kk + 1][0]; af[x][3] = pf[x][2 * kk + 1][1];
-        }
-        if (Q8) {
+          for (int x = 0; x < TERMS; ++x) {
+            if constexpr (WIDE) {
+              const uint32_t pa[4] = {pf[x][2 * kk][0], pf[x][2 * kk][E - 1], pf[x][2 * kk + 1][0], pf[x][2 * kk + 1][E - 1]};
+              TypeTraits<M>::mma(o[n], pa, f[0], f[1]);
+              TypeTraits<M>::mma(o[n + 1], pa, f[2], f[3]);
+            } else {
+              const uint32_t va[4] = {f[0], f[2], f[1], f[3]};
+              TypeTraits<M>::mma(o[n / 2], va, pf[x][2 * kk][0], pf[x][2 * kk + 1][0]);
+            }
+          }
+        };
+        if constexpr (Q8) {
           constexpr int WORDS = D / 32;           // words of four dims per token that a thread widens
           uint32_t w[4][WORDS];
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             const int row = kk * 16 + (j >> 1) * 8 + 2 * t + (j & 1);
-            if (WORDS == 4) {
+            if constexpr (WORDS == 4) {
               const uint4 v = *reinterpret_cast<const uint4*>(sv + S::at(row, g));
-              w[j][0] = v.x; w[j][1 % WORDS] = v.y; w[j][2 % WORDS] = v.z; w[j][3 % WORDS] = v.w;
+              w[j][0] = v.x; w[j][1] = v.y; w[j][2] = v.z; w[j][3] = v.w;
             } else {
               const uint2 v = *reinterpret_cast<const uint2*>(sv + S::at(row, g >> 1) + (g & 1) * 8);
-              w[j][0] = v.x; w[j][1 % WORDS] = v.y;
+              w[j][0] = v.x; w[j][1] = v.y;
             }
             if (CODE == XKV_CACHE_INT8)
 #pragma unroll
@@ -448,13 +558,7 @@ __global__ void __launch_bounds__(NT, 2) stream_kernel(const Args a) {
             for (int k = 0; k < 2; ++k) {        // dims 4i + 2k, + 1: bytes of two tokens side by side
               const uint32_t x = __byte_perm(w[0][i], w[1][i], k ? 0x7362u : 0x5140u);
               const uint32_t y = __byte_perm(w[2][i], w[3][i], k ? 0x7362u : 0x5140u);
-#pragma unroll
-              for (int e = 0; e < 2; ++e) {
-                const int n = 4 * i + 2 * k + e;
-                const uint32_t b0 = widen<CODE>(x, e), b1 = widen<CODE>(y, e);
-                TypeTraits<M>::mma(o[n], af[0], b0, b1);
-                if (TERMS == 2) TypeTraits<M>::mma(o[n], af[TERMS - 1], b0, b1);
-              }
+              product(4 * i + 2 * k, {widen<CODE>(x, 0), widen<CODE>(y, 0), widen<CODE>(x, 1), widen<CODE>(y, 1)});
             }
         } else {
           const int mi = lane >> 3, r = lane & 7;
@@ -465,30 +569,23 @@ __global__ void __launch_bounds__(NT, 2) stream_kernel(const Args a) {
             asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
                          : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3])
                          : "r"(smem_u32(sv) + S::at(row, n + (mi >> 1))) : "memory");
-            TypeTraits<M>::mma(o[n], af[0], v[0], v[1]);
-            TypeTraits<M>::mma(o[n + 1], af[0], v[2], v[3]);
+            product(n, v);
           }
         }
       }
-      // column of accumulator n, element e: 8-bit caches deal 16 (8) consecutive dims to the eight column groups
       while (bad) {
         const int tok = __ffsll((long long)bad) - 1;
         bad &= bad - 1;
-        const uint8_t* vr = vbase + (int64_t)(t0 + tok) * p.v_sl * S::ES;
+        const uint8_t* vr = vbase + (int64_t)(t0 + tok) * v_pitch;
 #pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          const int row = rb * RB + g + r * 8;
-          if (row >= a.rows || !sees(p, b, row % T_, t0 + tok, sp.first)) continue;
+        for (int n = 0; n < NO * E / 2; ++n)
 #pragma unroll
-          for (int n = 0; n < NO; ++n)
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              const int d = Q8 ? (2 * t + e) * NO + n : n * 8 + 2 * t + e;
-              const float x = Q8 ? __half2float(__half(__nv_cvt_fp8_to_halfraw(vr[d], __NV_E4M3)))
-                                 : to_float(reinterpret_cast<const M*>(vr)[d]);
-              if (!(fabsf(x) < CUDART_INF_F)) o[n][2 * r + e] += x;
-            }
-        }
+          for (int i = 0; i < 4; ++i) {
+            const int row = rb * RB + row_of(i), d = dim_of(n, i);
+            const float x = Q8 ? __half2float(__half(__nv_cvt_fp8_to_halfraw(vr[d], __NV_E4M3)))
+                               : to_float(reinterpret_cast<const M*>(vr)[d]);
+            if (!(fabsf(x) < CUDART_INF_F) && row < a.rows && sees(p, b, row % T_, t0 + tok, sp.first)) o[n][i] += x;
+          }
       }
       __syncwarp();       // every lane is done with the stage before the next copies into it
     }
@@ -498,20 +595,20 @@ __global__ void __launch_bounds__(NT, 2) stream_kernel(const Args a) {
     __syncthreads();
     constexpr int OS = D + 4;
     float* acc = reinterpret_cast<float*>(smem);               // [warp][row][OS]
-    float2* ml = reinterpret_cast<float2*>(qs);                // [warp][row]
+    float2* ml = reinterpret_cast<float2*>(qfrag);             // [warp][row]
     static_assert(NW * RB * OS * 4 <= NW * STAGES * S::STAGE, "the ring holds the partial outputs");
 #pragma unroll
+    for (int n = 0; n < NO * E / 2; ++n)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        acc[(warp * RB + row_of(i)) * OS + dim_of(n, i)] = o[n][i] * (Q8 ? unit_v[WIDE ? i >> 1 : i & 1] : 1.f);
+#pragma unroll
     for (int r = 0; r < 2; ++r) {
-      float sum = l[r].x + l[r].y;
-      sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-      sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-      float* row = acc + (warp * RB + g + r * 8) * OS;
-      const float f = Q8 ? unit_v[r] : 1.f;
+      float sum = WIDE ? l[r].x + l[r].y : r ? l[0].y : l[0].x;
 #pragma unroll
-      for (int n = 0; n < NO; ++n)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) row[Q8 ? (2 * t + e) * NO + n : n * 8 + 2 * t + e] = o[n][2 * r + e] * f;
-      if (t == 0) ml[warp * RB + g + r * 8] = make_float2(ref[r] == -CUDART_INF_F ? ref[r] : ref[r] - LIFT, sum);
+      for (int o = WIDE ? 1 : 4; o < (WIDE ? 4 : 32); o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      if ((WIDE ? t : g) == 0)
+        ml[warp * RB + (WIDE ? g + 8 * r : 2 * t + r)] = make_float2(ref[r] == -CUDART_INF_F ? ref[r] : ref[r] - LIFT, sum);
     }
     __syncthreads();
     const int live = min(RB, a.rows - rb * RB);
@@ -546,10 +643,10 @@ __global__ void __launch_bounds__(NT, 2) stream_kernel(const Args a) {
   }
 }
 
-template <typename T, int CODE, int D, int TERMS>
+template <typename T, int CODE, int D, int TERMS, int RB>
 int launch(const Args& a, cudaStream_t st) {
-  auto kern = stream_kernel<T, CODE, D, TERMS>;
-  constexpr int smem = Shape<T, CODE, D>::SMEM;
+  auto kern = stream_kernel<T, CODE, D, TERMS, RB>;
+  constexpr int smem = NW * STAGES * Shape<T, CODE, D>::STAGE + TERMS * Shape<T, CODE, D>::FRAGS + 16 * (int)sizeof(float2);
   if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) {
     cudaGetLastError();
     return XKV_ERR_LAUNCH;
@@ -558,12 +655,13 @@ int launch(const Args& a, cudaStream_t st) {
   return cudaGetLastError() == cudaSuccess ? XKV_OK : XKV_ERR_LAUNCH;
 }
 template <typename T, int CODE, int TERMS>
-int by_dim(const Args& a, cudaStream_t st) {
-  return a.p.head_dim == 128 ? launch<T, CODE, 128, TERMS>(a, st) : launch<T, CODE, 64, TERMS>(a, st);
+int by_shape(const Args& a, cudaStream_t st) {
+  if (a.p.head_dim == 128) return a.block_rows == 8 ? launch<T, CODE, 128, TERMS, 8>(a, st) : launch<T, CODE, 128, TERMS, 16>(a, st);
+  return a.block_rows == 8 ? launch<T, CODE, 64, TERMS, 8>(a, st) : launch<T, CODE, 64, TERMS, 16>(a, st);
 }
 template <typename T, int TERMS>
 int by_code(const Args& a, cudaStream_t st) {
-  return a.p.cache_code == XKV_CACHE_INT8 ? by_dim<T, XKV_CACHE_INT8, TERMS>(a, st) : by_dim<T, XKV_CACHE_E4M3, TERMS>(a, st);
+  return a.p.cache_code == XKV_CACHE_INT8 ? by_shape<T, XKV_CACHE_INT8, TERMS>(a, st) : by_shape<T, XKV_CACHE_E4M3, TERMS>(a, st);
 }
 
 bool rows_aligned(const void* ptr, int64_t sb, int64_t sh, int64_t sl, int es) {
@@ -588,15 +686,15 @@ bool tree_stream_supported(const xkv_tree_params& p) {
 void tree_stream_plan(const xkv_tree_params& p, TreePlan* pl) {
   pl->kernel = TreePlan::kStream;
   pl->name = "stream";
-  pl->block_rows = tree::RB;
+  pl->block_rows = pl->rows <= 8 ? 8 : 16;
   pl->unit_tokens = tree::NW * tree::HALF / (p.head_dim * (p.cache_code == XKV_CACHE_DENSE ? 2 : 1));
-  pl->slots = 2 * device_sm_count();            // two blocks per SM
+  pl->slots = (p.dtype == XKV_F32 ? tree::resident<2>() : tree::resident<1>()) * device_sm_count();
 }
 
 int tree_stream_decode(const tree::Args& a, cudaStream_t st) {
   using namespace tree;
   if (a.p.cache_code == XKV_CACHE_DENSE)
-    return a.p.dtype == XKV_BF16 ? by_dim<__nv_bfloat16, XKV_CACHE_DENSE, 1>(a, st) : by_dim<__half, XKV_CACHE_DENSE, 1>(a, st);
+    return a.p.dtype == XKV_BF16 ? by_shape<__nv_bfloat16, XKV_CACHE_DENSE, 1>(a, st) : by_shape<__half, XKV_CACHE_DENSE, 1>(a, st);
   if (a.p.dtype == XKV_BF16) return by_code<__nv_bfloat16, 1>(a, st);
   if (a.p.dtype == XKV_F16) return by_code<__half, 1>(a, st);
   return by_code<float, 2>(a, st);
