@@ -30,6 +30,7 @@ struct Args {
   float* part_o;           // [piece][block_rows][head_dim]
   float2* part_ml;         // [piece][block_rows]
   int* status;
+  int map_b[2], map_h[2];  // tensor maps of K and V: 0 where the sequences / KV heads share one (stride 0)
 };
 
 // Cache rows of one sequence: [0, first) is seen by every token, [first, len) holds the drafted tokens.
@@ -169,7 +170,7 @@ __device__ __forceinline__ bool next_piece(const Args& a, Walk& w, Piece& pc) {
 
 // ---- host side -------------------------------------------------------------------------------------------------
 struct TreePlan {
-  enum Kernel { kPortable, kStream } kernel;
+  enum Kernel { kPortable, kStream, kTc } kernel;
   const char* name;
   int rows, block_rows, unit_tokens, slots;      // slots: blocks of the kernel that the device holds at once
   int blocks, grid;
@@ -182,5 +183,10 @@ int tree_merge(const tree::Args& a, cudaStream_t st);
 bool tree_stream_supported(const xkv_tree_params& p);
 void tree_stream_plan(const xkv_tree_params& p, TreePlan* pl);
 int tree_stream_decode(const tree::Args& a, cudaStream_t st);
+
+// many query rows on tcgen05 (tree_tc_sm100.cu): what the stream kernel takes, 16-bit queries, more than 16 rows
+bool tree_tc_supported(const xkv_tree_params& p, int rows);
+void tree_tc_plan(const xkv_tree_params& p, TreePlan* pl);
+int tree_tc_decode(const tree::Args& a, cudaStream_t st);
 
 }  // namespace xkv

@@ -334,8 +334,12 @@ void portable_plan(const xkv_tree_params& p, TreePlan* pl) {
 
 bool make_plan(const xkv_tree_params& p, TreePlan* pl) {
   pl->rows = p.num_heads / p.num_kv_heads * p.num_tokens;
-  if (!(p.flags & XKV_FLAG_FORCE_GENERIC) && tree_stream_supported(p)) tree_stream_plan(p, pl);
-  else portable_plan(p, pl);
+  if (!(p.flags & XKV_FLAG_FORCE_GENERIC) && tree_stream_supported(p)) {
+    if (tree_tc_supported(p, pl->rows)) tree_tc_plan(p, pl);
+    else tree_stream_plan(p, pl);
+  } else {
+    portable_plan(p, pl);
+  }
   pl->blocks = ceil_div(pl->rows, pl->block_rows);
   const int64_t strips = (int64_t)p.batch * p.num_kv_heads * pl->blocks;
   if (strips > 0x7fffffff / 2) return false;
@@ -407,7 +411,8 @@ int xkv_tree_decode(const xkv_tree_params* p, void* ws, size_t ws_bytes, void* s
   a.part_ml = reinterpret_cast<float2*>(w + pl.off_ml);
   a.status = reinterpret_cast<int*>(w);
   int e;
-  if (pl.kernel == TreePlan::kStream) e = tree_stream_decode(a, st);
+  if (pl.kernel == TreePlan::kTc) e = tree_tc_decode(a, st);
+  else if (pl.kernel == TreePlan::kStream) e = tree_stream_decode(a, st);
   else if (p->dtype == XKV_F32) e = tree::portable<float>(a, st);
   else if (p->dtype == XKV_BF16) e = tree::portable<__nv_bfloat16>(a, st);
   else e = tree::portable<__half>(a, st);

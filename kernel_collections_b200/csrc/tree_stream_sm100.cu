@@ -4,7 +4,8 @@
 // rate and the pass is bound by HBM as long as the instructions per cache byte stay low.  Hence:
 //  * Every warp is on its own: it copies its 4 KB of K and of V (32 tokens of 128 codes, 16 of 128 halves) into a private
 //    two-stage ring with cp.async and meets the other warps only at the end of a piece.  No block barrier in the loop,
-//    nothing to wait for but its own copies.
+//    nothing to wait for but its own copies.  Eight warps in one block per SM, one tile ahead: twelve warps, or eight with
+//    two tiles ahead, have more bytes in flight and reach less of HBM (4 x 131071 rows of 8 heads: 189 us against 200).
 //  * With at most 8 query rows the tokens (and, for P.V, the dims) are the 16 rows of the MMA and the queries its 8 columns:
 //    half the MMAs, accumulators and exponentials of the 16-row form, which pads the queries to 16.  The weights then
 //    turn from accumulator to operand layout by movmatrix.
@@ -31,7 +32,7 @@ namespace tree {
 using namespace sm100;
 namespace {
 
-constexpr int NW = 4, NT = NW * 32, STAGES = 2, HALF = 4096;   // HALF: bytes of K (or V) per warp and stage
+constexpr int NW = 8, NT = NW * 32, STAGES = 2, HALF = 4096;   // HALF: bytes of K (or V) per warp and stage
 
 template <typename T> __device__ __forceinline__ float to_float(T v) { return TypeTraits<T>::to_f(v); }
 template <> __device__ __forceinline__ float to_float<float>(float v) { return v; }
@@ -118,13 +119,10 @@ struct Shape {
   static __device__ __forceinline__ int dim0(int s, int t) { return piece(s / KPC, t) * (16 / ES) + (s % KPC) * 4; }
 };
 
-// Blocks per SM.
-template <int TERMS> constexpr int resident() { return TERMS == 1 ? 3 : 2; }
-
 // RB query rows per strip.  A thread's two rows and its tokens of every 8: RB == 16: rows g, g + 8 and tokens 2t, 2t + 1;
 // RB == 8: rows 2t, 2t + 1 and token g.
 template <typename T, int CODE, int D, int TERMS, int RB>
-__global__ void __launch_bounds__(NT, resident<TERMS>()) stream_kernel(const Args a) {
+__global__ void __launch_bounds__(NT, 1) stream_kernel(const Args a) {
   using S = Shape<T, CODE, D>;
   constexpr bool Q8 = CODE != XKV_CACHE_DENSE, WIDE = RB == 16;
   constexpr bool RAISED = CODE == XKV_CACHE_INT8 && TERMS == 1;       // keys enter the product 1152 above their value
@@ -688,7 +686,7 @@ void tree_stream_plan(const xkv_tree_params& p, TreePlan* pl) {
   pl->name = "stream";
   pl->block_rows = pl->rows <= 8 ? 8 : 16;
   pl->unit_tokens = tree::NW * tree::HALF / (p.head_dim * (p.cache_code == XKV_CACHE_DENSE ? 2 : 1));
-  pl->slots = (p.dtype == XKV_F32 ? tree::resident<2>() : tree::resident<1>()) * device_sm_count();
+  pl->slots = device_sm_count();
 }
 
 int tree_stream_decode(const tree::Args& a, cudaStream_t st) {
