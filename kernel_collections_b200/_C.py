@@ -262,27 +262,34 @@ def run_decode(params: DecodeParams, device: torch.device, entry: str = "xkv_dec
             raise_on_status(ws.data_ptr(), stream, entry)
 
 
-def launch(fn: str, block: bytes, device: torch.device):
-    """Run entry point `fn` (a packed parameter block and the stream) on `device`'s current stream."""
-    lib = load()
-    idx = _device_of(device)
+def device_index(*tensors) -> int:
+    """Index of the one CUDA device that all tensors live on; raises as require_cuda does where there is none.  Integer
+    comparisons only: a launch-bound call notices more."""
+    idx = tensors[0].get_device()
+    for t in tensors:
+        if t.get_device() != idx or idx < 0:
+            require_cuda(*tensors)
+    return idx
+
+
+def launch(fn: str, block: bytes, idx: int):
+    """Run entry point `fn` (a packed parameter block and the stream) on device `idx`'s current stream."""
     if idx == torch.cuda.current_device():
-        rc = getattr(lib, fn)(block, torch._C._cuda_getCurrentRawStream(idx))
+        rc = getattr(_lib or load(), fn)(block, torch._C._cuda_getCurrentRawStream(idx))
+        if rc:
+            check(rc, fn)
     else:
         with torch.cuda.device(idx):
-            rc = getattr(lib, fn)(block, torch._C._cuda_getCurrentRawStream(idx))
-    if rc:
-        check(rc, fn)
+            launch(fn, block, idx)
 
 
-def run_tree_decode(block: bytes, device: torch.device, check_status=None):
+def run_tree_decode(block: bytes, device: torch.device, idx: int, check_status=None):
     """xkv_tree_decode with a workspace of the call's own: the caching allocator hands it on in stream order, and a
-    captured call keeps its workspace in its graph's pool, so no two graphs or streams share one."""
-    idx = _device_of(device)
+    captured call keeps its workspace in its graph's pool, so no two graphs, streams or threads share one."""
     if idx != torch.cuda.current_device():
         with torch.cuda.device(idx):
-            return run_tree_decode(block, device, check_status)
-    lib = load()
+            return run_tree_decode(block, device, idx, check_status)
+    lib = _lib or load()
     nbytes = lib.xkv_tree_decode_workspace_bytes(block)
     if nbytes == 0:
         # let the entry point produce the precise status

@@ -285,41 +285,43 @@ def latent_append(latent, new_rows, proj, position):
     return latent
 
 
-def _tree_decode(query, k, v, k_scales, v_scales, code, tree_mask, sm_scale, kv_lens, num_splits, force_generic,
+def _tree_decode(query, idx, KVH, L, k, ks, v, vs, scales, code, tree_mask, sm_scale, kv_lens, num_splits, force_generic,
                  check_status):
-    """Shared by the two tree entry points: k / v (bsz, num_kv_heads, kv_len, head_dim), scales or None."""
+    """Shared by the two tree entry points: k / v (bsz, KVH, L, head_dim) with strides ks / vs, `scales` the pointers and
+    strides of the key and value scales."""
     b, H, T, D = query.shape
-    KVH, L = k.shape[1], k.shape[2]
     if H % KVH != 0:
         raise ValueError("num_heads must be divisible by num_kv_heads")
     tm_ptr, tm_sb, tm_st = 0, 0, 0
     if tree_mask is not None:
-        _C.require_cuda(query, tree_mask)
-        if tree_mask.dtype != torch.bool or tuple(tree_mask.shape) not in ((T, T), (b, T, T)):
+        _C.device_index(query, tree_mask)
+        shape = tree_mask.shape
+        if tree_mask.dtype != torch.bool or (shape != (T, T) and shape != (b, T, T)):
             raise ValueError(f"tree_mask must be a bool tensor of shape ({T}, {T}) or ({b}, {T}, {T}); got "
-                             f"{tree_mask.dtype} {tuple(tree_mask.shape)}")
-        if tree_mask.stride(-1) != 1 and T != 1:
+                             f"{tree_mask.dtype} {tuple(shape)}")
+        st = tree_mask.stride()
+        if st[-1] != 1 and T != 1:
             tree_mask = tree_mask.contiguous()
-        tm_ptr, tm_st = tree_mask.data_ptr(), tree_mask.stride(-2)
-        tm_sb = tree_mask.stride(0) if tree_mask.dim() == 3 else 0
+            st = tree_mask.stride()
+        tm_ptr, tm_st, tm_sb = tree_mask.data_ptr(), st[-2], st[0] if len(shape) == 3 else 0
     len_ptr = 0
     if kv_lens is not None:
-        _C.require_cuda(query, kv_lens)
-        if kv_lens.dtype != torch.int32 or tuple(kv_lens.shape) != (b,) or not kv_lens.is_contiguous():
+        _C.device_index(query, kv_lens)
+        if kv_lens.dtype != torch.int32 or kv_lens.dim() != 1 or kv_lens.numel() != b or not kv_lens.is_contiguous():
             raise ValueError("kv_lens must be a contiguous int32 tensor of shape (batch,)")
         len_ptr = kv_lens.data_ptr()
-    q = query if query.stride(3) == 1 or D == 1 else query.contiguous()
-    out = torch.empty((b, H, T, D), dtype=q.dtype, device=q.device)
-    qs, ks, vs = q.stride(), k.stride(), v.stride()
-    kp = vp = (0, 0, 0)
-    if k_scales is not None:
-        kp = (k_scales.data_ptr(), k_scales.stride(0), k_scales.stride(1))
-        vp = (v_scales.data_ptr(), v_scales.stride(0), v_scales.stride(1))
+    dtype = _C.dtype_code(query)
+    q, qs = query, query.stride()
+    if qs[3] != 1 and D != 1:
+        q = query.contiguous()
+        qs = q.stride()
+    device = q.device
+    out = torch.empty_like(q) if q.is_contiguous() else torch.empty((b, H, T, D), dtype=q.dtype, device=device)
     _C.run_tree_decode(_C.TREE_PARAMS.pack(
-        _C.dtype_code(q), code, _C.FLAG_FORCE_GENERIC if force_generic else 0, b, H, KVH, T, L, D, num_splits,
+        dtype, code, _C.FLAG_FORCE_GENERIC if force_generic else 0, b, H, KVH, T, L, D, num_splits,
         D ** -0.5 if sm_scale is None else sm_scale, len_ptr, tm_ptr, tm_sb, tm_st, q.data_ptr(), qs[0], qs[1], qs[2],
-        k.data_ptr(), ks[0], ks[1], ks[2], v.data_ptr(), vs[0], vs[1], vs[2], *kp, *vp, out.data_ptr(), H * T * D, D),
-        q.device, check_status)
+        k.data_ptr(), ks[0], ks[1], ks[2], v.data_ptr(), vs[0], vs[1], vs[2], *scales, out.data_ptr(), H * T * D, D),
+        device, idx, check_status)
     return out
 
 
@@ -333,17 +335,24 @@ def group_query_attention_tree(query, key, value, tree_mask=None, *, sm_scale=No
     those, and drafted token u where tree_mask[t, u] (bool, (T, T) or (bsz, T, T); default: u <= t, a chain).  What a
     token does not see does not reach it, NaN and infinities included; a token that sees nothing gives zeros.
     Logits are multiplied by sm_scale (default 1 / sqrt(head_dim)).  Returns (bsz, num_heads, T, head_dim)."""
-    _C.require_cuda(query, key, value)
-    if query.dim() != 4 or key.dim() != 4 or key.shape != value.shape:
+    idx = _C.device_index(query, key, value)
+    qshape, shape = query.shape, key.shape
+    if len(qshape) != 4 or len(shape) != 4 or shape != value.shape:
         raise ValueError("query (bsz, num_heads, T, head_dim) and key / value (bsz, num_kv_heads, kv_len, head_dim) expected; "
-                         f"got {tuple(query.shape)}, {tuple(key.shape)} and {tuple(value.shape)}")
-    if key.shape[0] != query.shape[0] or key.shape[3] != query.shape[3]:
-        raise ValueError(f"batch or head_dim mismatch between query {tuple(query.shape)} and key {tuple(key.shape)}")
+                         f"got {tuple(qshape)}, {tuple(shape)} and {tuple(value.shape)}")
+    if shape[0] != qshape[0] or shape[3] != qshape[3]:
+        raise ValueError(f"batch or head_dim mismatch between query {tuple(qshape)} and key {tuple(shape)}")
     if key.dtype != query.dtype or value.dtype != query.dtype:
         raise ValueError("all tensors of one call must share a dtype")
-    k, v = (t if t.stride(3) == 1 or t.shape[3] == 1 else t.contiguous() for t in (key, value))
-    return _tree_decode(query, k, v, None, None, _C.CACHE_DENSE, tree_mask, sm_scale, kv_lens, num_splits, force_generic,
-                        check_status)
+    ks, vs = key.stride(), value.stride()
+    if ks[3] != 1 and shape[3] != 1:
+        key = key.contiguous()
+        ks = key.stride()
+    if vs[3] != 1 and shape[3] != 1:
+        value = value.contiguous()
+        vs = value.stride()
+    return _tree_decode(query, idx, shape[1], shape[2], key, ks, value, vs, (0, 0, 0, 0, 0, 0), _C.CACHE_DENSE, tree_mask,
+                        sm_scale, kv_lens, num_splits, force_generic, check_status)
 
 
 def group_query_attention_quantized(query, cache, tree_mask=None, *, sm_scale=None, kv_lens=None, num_splits=0,
@@ -352,12 +361,14 @@ def group_query_attention_quantized(query, cache, tree_mask=None, *, sm_scale=No
     and the scales applied to logits and probabilities.  query (bsz, num_heads, T, head_dim), T = 1 for a plain decode
     step, float32, bfloat16 or float16.  kv_lens, tree_mask and sm_scale as in group_query_attention_tree (kv_lens
     defaults to the cache's capacity).  Returns (bsz, num_heads, T, head_dim)."""
-    b, KVH, cap, D, code = quant_cache.check_cache(cache)
-    _C.require_cuda(cache.key_codes, query)
-    if query.dim() != 4 or query.shape[0] != b or query.shape[3] != D:
-        raise ValueError(f"query must be ({b}, num_heads, T, {D}); got {tuple(query.shape)}")
-    return _tree_decode(query, cache.key_codes, cache.value_codes, cache.key_scales, cache.value_scales, code, tree_mask,
-                        sm_scale, kv_lens, num_splits, force_generic, check_status)
+    (idx, b, KVH, cap, D, code), (ks, vs, kss, vss) = quant_cache.check_cache(cache)
+    _C.device_index(cache.key_codes, query)
+    shape = query.shape
+    if len(shape) != 4 or shape[0] != b or shape[3] != D:
+        raise ValueError(f"query must be ({b}, num_heads, T, {D}); got {tuple(shape)}")
+    scales = (cache.key_scales.data_ptr(), kss[0], kss[1], cache.value_scales.data_ptr(), vss[0], vss[1])
+    return _tree_decode(query, idx, KVH, cap, cache.key_codes, ks, cache.value_codes, vs, scales, code, tree_mask, sm_scale,
+                        kv_lens, num_splits, force_generic, check_status)
 
 
 def xkv_group_decode(queries, key_A, key_Bs, value, value_Bs=None, *, theta, sm_scale=None,

@@ -39,27 +39,30 @@ def quantized_cache(batch, num_kv_heads, capacity, head_dim, *, code="int8", dev
 
 
 def check_cache(cache):
-    """(batch, num_kv_heads, capacity, head_dim, code) of a cache whose tensors fit together; raises where they do not."""
+    """(device index, batch, num_kv_heads, capacity, head_dim, code) of a cache whose tensors fit together, and the
+    strides of key_codes, value_codes, key_scales and value_scales; raises where they do not."""
     kc, ks, vc, vs = cache.key_codes, cache.key_scales, cache.value_codes, cache.value_scales
-    _C.require_cuda(kc, ks, vc, vs)
+    idx = _C.device_index(kc, ks, vc, vs)
     code = _C.CACHE_CODES.get(kc.dtype)
     if code is None or vc.dtype != kc.dtype:
         raise ValueError(f"codes must be int8 or float8_e4m3fn, keys and values alike; got {kc.dtype} and {vc.dtype}")
-    if kc.dim() != 4 or vc.shape != kc.shape:
+    shape = kc.shape
+    if len(shape) != 4 or vc.shape != shape:
         raise ValueError(f"codes must be (bsz, num_kv_heads, capacity, head_dim); got {tuple(kc.shape)} and {tuple(vc.shape)}")
-    b, h, cap, d = kc.shape
-    if ks.dtype != torch.float32 or vs.dtype != torch.float32 or ks.shape != (b, h, cap) or vs.shape != (b, h, cap):
+    b, h, cap, d = shape
+    if ks.dtype != torch.float32 or vs.dtype != torch.float32 or ks.shape != shape[:3] or vs.shape != shape[:3]:
         raise ValueError(f"scales must be float32 ({b}, {h}, {cap}) tensors")
-    if (d > 1 and (kc.stride(3) != 1 or vc.stride(3) != 1)) or (cap > 1 and (ks.stride(2) != 1 or vs.stride(2) != 1)):
+    kcs, vcs, kss, vss = kc.stride(), vc.stride(), ks.stride(), vs.stride()
+    if (d > 1 and (kcs[3] != 1 or vcs[3] != 1)) or (cap > 1 and (kss[2] != 1 or vss[2] != 1)):
         raise ValueError("codes and scales need a contiguous last dim")
-    return b, h, cap, d, code
+    return (idx, b, h, cap, d, code), (kcs, vcs, kss, vss)
 
 
 def _start(position, b, like):
     """(int, pointer) of a first row given as an int or an int32 (bsz,) device tensor."""
     if isinstance(position, torch.Tensor):
-        _C.require_cuda(like, position)
-        if position.dtype != torch.int32 or tuple(position.shape) != (b,) or not position.is_contiguous():
+        _C.device_index(like, position)
+        if position.dtype != torch.int32 or position.dim() != 1 or position.numel() != b or not position.is_contiguous():
             raise ValueError("positions must be a contiguous int32 device tensor of shape (bsz,)")
         return 0, position.data_ptr()
     p = int(position)
@@ -68,14 +71,13 @@ def _start(position, b, like):
     return p, 0
 
 
-def _launch(entry, cache, dims, n, dtype, pos, pos_ptr, len_ptr, k, v):
-    b, h, cap, d, code = dims
-    kc, vc, ks, vs = cache.key_codes, cache.value_codes, cache.key_scales, cache.value_scales
-    a, c, e, f = k.stride(), v.stride(), kc.stride(), vc.stride()
+def _launch(entry, cache, dims, strides, n, dtype, pos, pos_ptr, len_ptr, k, a, v, c):
+    idx, b, h, cap, d, code = dims
+    kcs, vcs, kss, vss = strides
     _C.launch(entry, _C.CACHE_PARAMS.pack(
         dtype, code, b, h, n, cap, d, pos, pos_ptr, len_ptr, k.data_ptr(), a[0], a[1], a[2], v.data_ptr(), c[0], c[1], c[2],
-        kc.data_ptr(), e[0], e[1], e[2], vc.data_ptr(), f[0], f[1], f[2], ks.data_ptr(), ks.stride(0), ks.stride(1),
-        vs.data_ptr(), vs.stride(0), vs.stride(1)), kc.device)
+        cache.key_codes.data_ptr(), kcs[0], kcs[1], kcs[2], cache.value_codes.data_ptr(), vcs[0], vcs[1], vcs[2],
+        cache.key_scales.data_ptr(), kss[0], kss[1], cache.value_scales.data_ptr(), vss[0], vss[1]), idx)
 
 
 def quantized_cache_append(cache, key, value, position, *, lengths=None):
@@ -85,10 +87,11 @@ def quantized_cache_append(cache, key, value, position, *, lengths=None):
     tensor (bsz,): the cache row of each sequence's first token, the others follow it.  `lengths` (int32 (bsz,)): only
     the first lengths[b] tokens of sequence b are written (padded prompts).  Rows outside the cache are left alone.  A
     row with an infinity or a NaN reads back as NaN throughout."""
-    dims = check_cache(cache)
-    b, h, cap, d, _ = dims
-    _C.require_cuda(cache.key_codes, key, value)
-    if key.dim() != 4 or key.shape != value.shape or key.shape[0] != b or key.shape[1] != h or key.shape[3] != d:
+    dims, strides = check_cache(cache)
+    idx, b, h, cap, d, _ = dims
+    _C.device_index(cache.key_codes, key, value)
+    shape = key.shape
+    if len(shape) != 4 or shape != value.shape or shape[0] != b or shape[1] != h or shape[3] != d:
         raise ValueError(f"key and value must be ({b}, {h}, n, {d}); got {tuple(key.shape)} and {tuple(value.shape)}")
     if key.dtype != value.dtype:
         raise ValueError("all tensors of one call must share a dtype")
@@ -96,34 +99,40 @@ def quantized_cache_append(cache, key, value, position, *, lengths=None):
     pos, pos_ptr = _start(position, b, key)
     len_ptr = 0
     if lengths is not None:
-        _C.require_cuda(key, lengths)
+        _C.device_index(key, lengths)
         if lengths.dtype != torch.int32 or tuple(lengths.shape) != (b,) or not lengths.is_contiguous():
             raise ValueError("lengths must be a contiguous int32 device tensor of shape (bsz,)")
         len_ptr = lengths.data_ptr()
-    if key.numel() == 0 or cap == 0:
+    n = shape[2]
+    if n == 0 or cap == 0 or b * h * d == 0:
         return cache
-    k = key if key.stride(3) == 1 or d == 1 else key.contiguous()
-    v = value if value.stride(3) == 1 or d == 1 else value.contiguous()
-    _launch("xkv_cache_append", cache, dims, k.shape[2], dtype, pos, pos_ptr, len_ptr, k, v)
+    k, v, a, c = key, value, key.stride(), value.stride()
+    if a[3] != 1 and d != 1:
+        k = key.contiguous()
+        a = k.stride()
+    if c[3] != 1 and d != 1:
+        v = value.contiguous()
+        c = v.stride()
+    _launch("xkv_cache_append", cache, dims, strides, n, dtype, pos, pos_ptr, len_ptr, k, a, v, c)
     return cache
 
 
 def quantized_cache_read(cache, position, length, *, dtype=torch.bfloat16):
     """Rows [position, position + length) of the cache as dense (key, value), each (bsz, num_kv_heads, length, head_dim)
     of `dtype`: code * scale, rounded once.  `position` as in quantized_cache_append; rows outside the cache are zeros."""
-    dims = check_cache(cache)
-    b, h, cap, d, _ = dims
+    dims, strides = check_cache(cache)
+    idx, b, h, cap, d, _ = dims
     n = int(length)
     if n < 0:
         raise ValueError("length must not be negative")
     pos, pos_ptr = _start(position, b, cache.key_codes)
-    dev = cache.key_codes.device
-    k = torch.empty((b, h, n, d), dtype=dtype, device=dev)
-    v = torch.empty((b, h, n, d), dtype=dtype, device=dev)
+    k = torch.empty((b, h, n, d), dtype=dtype, device=cache.key_codes.device)
+    v = torch.empty_like(k)
     code = _C.dtype_code(k)
-    if k.numel() == 0:
+    if n == 0 or b * h * d == 0:
         return k, v
     if cap == 0:
         return k.zero_(), v.zero_()
-    _launch("xkv_cache_read", cache, dims, n, code, pos, pos_ptr, 0, k, v)
+    a = (h * n * d, n * d, d)
+    _launch("xkv_cache_read", cache, dims, strides, n, code, pos, pos_ptr, 0, k, a, v, a)
     return k, v

@@ -68,10 +68,6 @@ def rotary_frequencies(rotary_dim, theta=10000.0, *, scaling=None, factor=1.0, o
     return torch.tensor(freq, dtype=torch.float64, device=device), magnitude
 
 
-def _row_contig(t):
-    return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
-
-
 def rotary_embedding(query, key, inv_freq, position, *, interleaved=False, magnitude=1.0, out=None):
     """Turn queries and keys of new tokens to their positions; returns (query', key').
 
@@ -80,25 +76,33 @@ def rotary_embedding(query, key, inv_freq, position, *, interleaved=False, magni
     rotary_dim / 2) or, with `interleaved`, (2j, 2j + 1); the others are copied.  `position`: an int or an int32
     tensor (bsz,), the position of each sequence's first token with the others following it, or an int32 tensor (bsz,
     n) of every token's own (drafted trees).  `out`: a (query', key') pair to fill; it may be the inputs themselves."""
-    _C.require_cuda(query, key, inv_freq)
-    if query.dim() != 4:
-        raise ValueError(f"query must be (bsz, num_heads, n, head_dim); got {tuple(query.shape)}")
-    b, H, n, D = query.shape
-    if key is not None and (key.dim() != 4 or key.shape[0] != b or key.shape[2] != n or key.shape[3] != D):
-        raise ValueError(f"key must be ({b}, num_kv_heads, {n}, {D}); got {tuple(key.shape)}")
-    if key is not None and key.dtype != query.dtype:
-        raise ValueError("all tensors of one call must share a dtype")
+    shape = query.shape
+    if len(shape) != 4:
+        raise ValueError(f"query must be (bsz, num_heads, n, head_dim); got {tuple(shape)}")
+    b, H, n, D = shape
+    dt = query.dtype
+    if key is None:
+        idx, KVH = _C.device_index(query, inv_freq), 0
+    else:
+        idx = _C.device_index(query, key, inv_freq)
+        kshape = key.shape
+        if len(kshape) != 4 or kshape[0] != b or kshape[2] != n or kshape[3] != D:
+            raise ValueError(f"key must be ({b}, num_kv_heads, {n}, {D}); got {tuple(kshape)}")
+        if key.dtype != dt:
+            raise ValueError("all tensors of one call must share a dtype")
+        KVH = kshape[1]
     if inv_freq.dtype != torch.float64 or inv_freq.dim() != 1 or not inv_freq.is_contiguous():
         raise ValueError("inv_freq must be a contiguous float64 tensor of shape (rotary_dim / 2,)")
-    rot = 2 * inv_freq.shape[0]
+    rot = 2 * inv_freq.numel()
     if not 0 < rot <= D:
         raise ValueError(f"inv_freq holds {rot // 2} pairs; head_dim {D} has room for {D // 2}")
     pos_ptr, pos_i, psb, pst = 0, 0, 0, 0
     if isinstance(position, torch.Tensor):
-        _C.require_cuda(query, position)
-        if position.dtype != torch.int32 or tuple(position.shape) not in ((b,), (b, n)):
+        _C.device_index(query, position)
+        pshape = position.shape
+        if position.dtype != torch.int32 or pshape[0] != b or not (len(pshape) == 1 or (len(pshape) == 2 and pshape[1] == n)):
             raise ValueError("positions must be an int32 device tensor of shape (bsz,) or (bsz, n)")
-        if position.dim() == 2:
+        if len(pshape) == 2:
             position = position.contiguous()
             pst = 1 if n > 1 else 0
         psb = position.stride(0)
@@ -107,11 +111,22 @@ def rotary_embedding(query, key, inv_freq, position, *, interleaved=False, magni
         pos_i = int(position)
         if not -2 ** 31 <= pos_i < 2 ** 31:
             raise ValueError("position must fit 32 bits")
-    q, k = _row_contig(query), None if key is None else _row_contig(key)
+    q, qs = query, query.stride()
+    if qs[3] != 1 and D != 1:
+        q = query.contiguous()
+        qs = q.stride()
+    k, ks = key, (0, 0, 0, 0)
+    if key is not None:
+        ks = key.stride()
+        if ks[3] != 1 and D != 1:
+            k = key.contiguous()
+            ks = k.stride()
     if out is None:
-        qo, ko = torch.empty_like(q), None if k is None else torch.empty_like(k)
-        qo, ko = (t if t is None or t.stride(-1) == 1 or D == 1 else torch.empty(t.shape, dtype=t.dtype, device=t.device)
-                  for t in (qo, ko))
+        qo = torch.empty_like(q)
+        ko = None if k is None else torch.empty_like(k)
+        if (qo.stride(3) != 1 and D != 1) or (ko is not None and ko.stride(3) != 1 and D != 1):
+            qo = torch.empty(shape, dtype=dt, device=q.device)
+            ko = None if k is None else torch.empty(k.shape, dtype=dt, device=q.device)
     else:
         qo, ko = out
         if (ko is None) != (key is None):
@@ -119,18 +134,16 @@ def rotary_embedding(query, key, inv_freq, position, *, interleaved=False, magni
         for o, t in ((qo, query), (ko, key)):
             if o is None:
                 continue
-            _C.require_cuda(query, o)
-            if o.shape != t.shape or o.dtype != t.dtype or (o.stride(-1) != 1 and D != 1):
+            _C.device_index(query, o)
+            if o.shape != t.shape or o.dtype != dt or (o.stride(3) != 1 and D != 1):
                 raise ValueError("outputs must have the inputs' shapes and dtype and a contiguous last dim")
     if query.numel() == 0:
         return qo, ko
-    qs, qt = q.stride(), qo.stride()
-    ks = kt = (0, 0, 0, 0)
+    qt, kt, kp, kop = qo.stride(), (0, 0, 0, 0), 0, 0
     if k is not None:
-        ks, kt = k.stride(), ko.stride()
+        kt, kp, kop = ko.stride(), k.data_ptr(), ko.data_ptr()
     _C.launch("xkv_rotary", _C.ROTARY_PARAMS.pack(
-        _C.dtype_code(q), b, H, 0 if k is None else k.shape[1], n, D, rot, 1 if interleaved else 0, pos_i, magnitude,
-        pos_ptr, psb, pst, inv_freq.data_ptr(),
-        q.data_ptr(), qs[0], qs[1], qs[2], 0 if k is None else k.data_ptr(), ks[0], ks[1], ks[2],
-        qo.data_ptr(), qt[0], qt[1], qt[2], 0 if k is None else ko.data_ptr(), kt[0], kt[1], kt[2]), q.device)
+        _C.dtype_code(q), b, H, KVH, n, D, rot, 1 if interleaved else 0, pos_i, magnitude, pos_ptr, psb, pst,
+        inv_freq.data_ptr(), q.data_ptr(), qs[0], qs[1], qs[2], kp, ks[0], ks[1], ks[2],
+        qo.data_ptr(), qt[0], qt[1], qt[2], kop, kt[0], kt[1], kt[2]), idx)
     return qo, ko
