@@ -3,7 +3,8 @@
 // One row (token, KV head) is reduced to its largest magnitude, scaled and rounded: scale = top * (1 / C), code =
 // rn(x * (C * (1 / top))), every operation rounded to fp32.  Both directions move every byte once and are bound by HBM for long stretches and by the launch for single
 // tokens.  A row is held in registers by a power-of-two group of lanes (16 bytes per lane and access), so the
-// reduction is a few shuffles and nothing is read twice; keys and values are the two halves of the grid.
+// reduction is a few shuffles and nothing is read twice.  Sequence and head come from the block's indices: one 64-bit
+// division per row costs more than the row's arithmetic.
 #include "xkv_internal.h"
 #include <cuda_fp8.h>
 #include <math_constants.h>
@@ -36,99 +37,125 @@ template <int CODE> __device__ __forceinline__ float decode(uint8_t c) {
   return __half2float(__half(__nv_cvt_fp8_to_halfraw(c, __NV_E4M3)));
 }
 
-struct Row {
-  int b, h, t;
-  int64_t at;      // cache row
+// A block works on one (sequence, KV head) of the keys or of the values: grid (2 x token chunks, KV heads, sequences).
+// `lanes` (a power of two, at most 32) lanes hold one row; a thread has its accesses of U rows in flight.
+struct Place {
+  int64_t start;      // cache row of token 0
+  int tokens;         // of this sequence
+  bool values;
+  int group, groups, lane;
 };
-__device__ __forceinline__ Row row_of(const xkv_cache_params& p, int64_t r) {
-  Row w;
-  const int64_t bh = r / p.num_tokens;
-  w.t = (int)(r - bh * p.num_tokens);
-  w.b = (int)(bh / p.num_kv_heads);
-  w.h = (int)(bh - (int64_t)w.b * p.num_kv_heads);
-  w.at = (int64_t)(p.positions ? p.positions[w.b] : p.position) + w.t;
+__device__ __forceinline__ Place place_of(const xkv_cache_params& p, int lanes) {
+  Place w;
+  const int b = blockIdx.z;
+  w.values = blockIdx.x & 1;
+  w.start = p.positions ? p.positions[b] : p.position;
+  w.tokens = p.num_tokens;
+  w.groups = NT / lanes;
+  w.group = threadIdx.x / lanes;
+  w.lane = threadIdx.x & (lanes - 1);
   return w;
 }
 
-// NV accesses of V elements per lane; `lanes` (a power of two, at most 32) lanes hold one row.
-template <typename T, int CODE, int V, int NV>
-__global__ void __launch_bounds__(NT) append_kernel(const xkv_cache_params p, int64_t rows, int lanes) {
-  const int lane = threadIdx.x & (lanes - 1);
-  const int64_t r = (int64_t)blockIdx.x * (NT / lanes) + threadIdx.x / lanes;
-  const bool values = blockIdx.y != 0;
-  Row w = {0, 0, 0, -1};
-  bool live = r < rows;
-  if (live) {
-    w = row_of(p, r);
-    live = w.at >= 0 && w.at < p.capacity && (!p.lengths || w.t < p.lengths[w.b]);
+// NV accesses of V elements per lane and row.
+template <typename T, int CODE, int V, int NV, int U>
+__global__ void __launch_bounds__(NT) append_kernel(const xkv_cache_params p, int lanes) {
+  const int h = blockIdx.y, b = blockIdx.z;
+  Place w = place_of(p, lanes);
+  if (p.lengths) w.tokens = min(w.tokens, p.lengths[b]);
+  const int t0 = (blockIdx.x >> 1) * (w.groups * U) + w.group;
+  const int64_t st = w.values ? p.v_st : p.k_st;
+  const T* src = (w.values ? static_cast<const T*>(p.v) + b * p.v_sb + h * p.v_sh : static_cast<const T*>(p.k) + b * p.k_sb + h * p.k_sh);
+  Vec<T, V> x[U][NV];
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const int t = t0 + u * w.groups;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int d = (i * lanes + w.lane) * V;
+      if (t < w.tokens && d < p.head_dim) x[u][i] = *reinterpret_cast<const Vec<T, V>*>(src + t * st + d);
+    }
   }
-  const T* src = static_cast<const T*>(values ? p.v : p.k) +
-                 (values ? w.b * p.v_sb + w.h * p.v_sh + w.t * p.v_st : w.b * p.k_sb + w.h * p.k_sh + w.t * p.k_st);
-  Vec<T, V> x[NV];
-  float top = 0.f;
-  bool odd = false;       // an infinity or a NaN
+  uint8_t* codes = w.values ? static_cast<uint8_t*>(p.v_codes) + b * p.vc_sb + h * p.vc_sh : static_cast<uint8_t*>(p.k_codes) + b * p.kc_sb + h * p.kc_sh;
+  float* scales = w.values ? p.v_scales + b * p.vs_sb + h * p.vs_sh : p.k_scales + b * p.ks_sb + h * p.ks_sh;
+  const int64_t sl = w.values ? p.vc_sl : p.kc_sl;
 #pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    const int d = (i * lanes + lane) * V;
-    if (live && d < p.head_dim) {
-      x[i] = *reinterpret_cast<const Vec<T, V>*>(src + d);
+  for (int u = 0; u < U; ++u) {
+    const int t = t0 + u * w.groups;
+    const int64_t at = w.start + t;
+    const bool live = t < w.tokens && at >= 0 && at < p.capacity;
+    float top = 0.f;
+    bool odd = false;       // an infinity or a NaN
 #pragma unroll
-      for (int e = 0; e < V; ++e) {
-        const float m = fabsf(to_f(x[i].x[e]));
-        odd |= !(m <= 3.402823466e38f);
-        top = fmaxf(top, m);
+    for (int i = 0; i < NV; ++i) {
+      const int d = (i * lanes + w.lane) * V;
+      if (t < w.tokens && d < p.head_dim) {
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+          const float m = fabsf(to_f(x[u][i].x[e]));
+          odd |= !(m <= 3.402823466e38f);
+          top = fmaxf(top, m);
+        }
       }
     }
-  }
-  if (odd) top = CUDART_INF_F;       // fmaxf passes a NaN over, an infinity survives it
-  for (int o = lanes >> 1; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-  if (!live) return;
-  const bool finite = top < CUDART_INF_F;
-  float scale = __fmul_rn(top, 1.0f / largest<CODE>());
-  float per = 0.f;
-  if (!finite) scale = CUDART_NAN_F;
-  else if (scale < 1.17549435e-38f) scale = 0.f;
-  else per = __fmul_rn(largest<CODE>(), __frcp_rn(top));
-  uint8_t* dst = static_cast<uint8_t*>(values ? p.v_codes : p.k_codes) +
-                 (values ? w.b * p.vc_sb + w.h * p.vc_sh + w.at * p.vc_sl : w.b * p.kc_sb + w.h * p.kc_sh + w.at * p.kc_sl);
+    if (odd) top = CUDART_INF_F;       // fmaxf passes a NaN over, an infinity survives it
+    for (int o = lanes >> 1; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    if (!live) continue;
+    const bool finite = top < CUDART_INF_F;
+    float scale = __fmul_rn(top, 1.0f / largest<CODE>());
+    float per = 0.f;
+    if (!finite) scale = CUDART_NAN_F;
+    else if (scale < 1.17549435e-38f) scale = 0.f;
+    else per = __fmul_rn(largest<CODE>(), __frcp_rn(top));
 #pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    const int d = (i * lanes + lane) * V;
-    if (d < p.head_dim) {
-      Vec<uint8_t, V> c;
+    for (int i = 0; i < NV; ++i) {
+      const int d = (i * lanes + w.lane) * V;
+      if (d < p.head_dim) {
+        Vec<uint8_t, V> c;
 #pragma unroll
-      for (int e = 0; e < V; ++e) c.x[e] = finite ? encode<CODE>(to_f(x[i].x[e]) * per) : 0;
-      *reinterpret_cast<Vec<uint8_t, V>*>(dst + d) = c;
+        for (int e = 0; e < V; ++e) c.x[e] = finite ? encode<CODE>(to_f(x[u][i].x[e]) * per) : 0;
+        *reinterpret_cast<Vec<uint8_t, V>*>(codes + at * sl + d) = c;
+      }
     }
-  }
-  if (lane == 0) {
-    if (values) p.v_scales[w.b * p.vs_sb + w.h * p.vs_sh + w.at] = scale;
-    else p.k_scales[w.b * p.ks_sb + w.h * p.ks_sh + w.at] = scale;
+    if (w.lane == 0) scales[at] = scale;
   }
 }
 
-template <typename T, int CODE, int V>
-__global__ void __launch_bounds__(NT) read_kernel(const xkv_cache_params p, int64_t rows, int lanes) {
-  const int lane = threadIdx.x & (lanes - 1);
-  const int64_t r = (int64_t)blockIdx.x * (NT / lanes) + threadIdx.x / lanes;
-  if (r >= rows) return;
-  const bool values = blockIdx.y != 0;
-  const Row w = row_of(p, r);
-  const bool live = w.at >= 0 && w.at < p.capacity;
-  const int64_t at = live ? w.at : 0;
-  const uint8_t* src = static_cast<const uint8_t*>(values ? p.v_codes : p.k_codes) +
-                       (values ? w.b * p.vc_sb + w.h * p.vc_sh + at * p.vc_sl : w.b * p.kc_sb + w.h * p.kc_sh + at * p.kc_sl);
-  const float scale = !live ? 0.f : values ? p.v_scales[w.b * p.vs_sb + w.h * p.vs_sh + at]
-                                           : p.k_scales[w.b * p.ks_sb + w.h * p.ks_sh + at];
-  T* dst = static_cast<T*>(values ? p.v : p.k) +
-           (values ? w.b * p.v_sb + w.h * p.v_sh + w.t * p.v_st : w.b * p.k_sb + w.h * p.k_sh + w.t * p.k_st);
-  for (int d = lane * V; d < p.head_dim; d += lanes * V) {
-    Vec<uint8_t, V> c = {};
-    if (live) c = *reinterpret_cast<const Vec<uint8_t, V>*>(src + d);
-    Vec<T, V> x;
+template <typename T, int CODE, int V, int U>
+__global__ void __launch_bounds__(NT) read_kernel(const xkv_cache_params p, int lanes) {
+  const int h = blockIdx.y, b = blockIdx.z;
+  const Place w = place_of(p, lanes);
+  const int t0 = (blockIdx.x >> 1) * (w.groups * U) + w.group;
+  const uint8_t* codes = w.values ? static_cast<const uint8_t*>(p.v_codes) + b * p.vc_sb + h * p.vc_sh
+                                  : static_cast<const uint8_t*>(p.k_codes) + b * p.kc_sb + h * p.kc_sh;
+  const float* scales = w.values ? p.v_scales + b * p.vs_sb + h * p.vs_sh : p.k_scales + b * p.ks_sb + h * p.ks_sh;
+  const int64_t sl = w.values ? p.vc_sl : p.kc_sl, st = w.values ? p.v_st : p.k_st;
+  T* dst = w.values ? static_cast<T*>(p.v) + b * p.v_sb + h * p.v_sh : static_cast<T*>(p.k) + b * p.k_sb + h * p.k_sh;
+  for (int d = w.lane * V; d < p.head_dim; d += lanes * V) {
+    Vec<uint8_t, V> c[U];
+    float scale[U];
 #pragma unroll
-    for (int e = 0; e < V; ++e) x.x[e] = live ? from_f<T>(decode<CODE>(c.x[e]) * scale) : from_f<T>(0.f);
-    *reinterpret_cast<Vec<T, V>*>(dst + d) = x;
+    for (int u = 0; u < U; ++u) {
+      const int t = t0 + u * w.groups;
+      const int64_t at = w.start + t;
+      c[u] = {};
+      scale[u] = 0.f;
+      if (t < w.tokens && at >= 0 && at < p.capacity) {
+        c[u] = *reinterpret_cast<const Vec<uint8_t, V>*>(codes + at * sl + d);
+        scale[u] = scales[at];
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int t = t0 + u * w.groups;
+      if (t >= w.tokens) break;
+      const int64_t at = w.start + t;
+      const bool live = at >= 0 && at < p.capacity;
+      Vec<T, V> x;
+#pragma unroll
+      for (int e = 0; e < V; ++e) x.x[e] = from_f<T>(live ? decode<CODE>(c[u].x[e]) * scale[u] : 0.f);
+      *reinterpret_cast<Vec<T, V>*>(dst + t * st + d) = x;
+    }
   }
 }
 
@@ -145,26 +172,43 @@ int lanes_for(int accesses) {      // per row
   return lanes;
 }
 
+// rows in flight per thread: four where there are tokens enough to keep every SM busy all the same
+template <int U>
+bool grid_of(const xkv_cache_params& p, int lanes, dim3* grid) {
+  const int64_t chunks = ((int64_t)p.num_tokens + NT / lanes * U - 1) / (NT / lanes * U);
+  if (chunks > 0x3fffffff || p.num_kv_heads > 65535 || p.batch > 65535) return false;
+  *grid = dim3((unsigned)(2 * chunks), (unsigned)p.num_kv_heads, (unsigned)p.batch);
+  return true;
+}
+bool many_tokens(const xkv_cache_params& p, int lanes) {
+  return (int64_t)p.num_tokens * p.num_kv_heads * p.batch * 2 * lanes >= (int64_t)device_sm_count() * 2048 * 4;
+}
+
+template <typename T, int CODE, int V, int NV, int U>
+int append_u(const xkv_cache_params& p, int lanes, cudaStream_t st) {
+  dim3 grid;
+  if (!grid_of<U>(p, lanes, &grid)) return XKV_ERR_UNSUPPORTED;
+  append_kernel<T, CODE, V, NV, U><<<grid, NT, 0, st>>>(p, lanes);
+  return cudaGetLastError() == cudaSuccess ? XKV_OK : XKV_ERR_LAUNCH;
+}
 template <typename T, int CODE, int V>
 int append_v(const xkv_cache_params& p, cudaStream_t st) {
-  const int64_t rows = (int64_t)p.batch * p.num_kv_heads * p.num_tokens;
   const int accesses = ceil_div(p.head_dim, V), lanes = lanes_for(accesses), nv = ceil_div(accesses, lanes);
-  const int64_t gx = (rows + NT / lanes - 1) / (NT / lanes);
-  if (gx > 0x7fffffff) return XKV_ERR_UNSUPPORTED;
-  const dim3 grid((unsigned)gx, 2);
-  if (nv == 1) append_kernel<T, CODE, V, 1><<<grid, NT, 0, st>>>(p, rows, lanes);
-  else if (nv <= 4) append_kernel<T, CODE, V, 4><<<grid, NT, 0, st>>>(p, rows, lanes);
-  else append_kernel<T, CODE, V, 32><<<grid, NT, 0, st>>>(p, rows, lanes);   // head_dim <= 1024 = 32 lanes x 32
+  if (nv == 1) return many_tokens(p, lanes) ? append_u<T, CODE, V, 1, 4>(p, lanes, st) : append_u<T, CODE, V, 1, 1>(p, lanes, st);
+  if (nv <= 4) return append_u<T, CODE, V, 4, 1>(p, lanes, st);
+  return append_u<T, CODE, V, 32, 1>(p, lanes, st);       // head_dim <= 1024 = 32 lanes x 32
+}
+template <typename T, int CODE, int V, int U>
+int read_u(const xkv_cache_params& p, int lanes, cudaStream_t st) {
+  dim3 grid;
+  if (!grid_of<U>(p, lanes, &grid)) return XKV_ERR_UNSUPPORTED;
+  read_kernel<T, CODE, V, U><<<grid, NT, 0, st>>>(p, lanes);
   return cudaGetLastError() == cudaSuccess ? XKV_OK : XKV_ERR_LAUNCH;
 }
 template <typename T, int CODE, int V>
 int read_v(const xkv_cache_params& p, cudaStream_t st) {
-  const int64_t rows = (int64_t)p.batch * p.num_kv_heads * p.num_tokens;
   const int lanes = lanes_for(ceil_div(p.head_dim, V));
-  const int64_t gx = (rows + NT / lanes - 1) / (NT / lanes);
-  if (gx > 0x7fffffff) return XKV_ERR_UNSUPPORTED;
-  read_kernel<T, CODE, V><<<dim3((unsigned)gx, 2), NT, 0, st>>>(p, rows, lanes);
-  return cudaGetLastError() == cudaSuccess ? XKV_OK : XKV_ERR_LAUNCH;
+  return many_tokens(p, lanes) ? read_u<T, CODE, V, 4>(p, lanes, st) : read_u<T, CODE, V, 1>(p, lanes, st);
 }
 
 template <typename T, int CODE>

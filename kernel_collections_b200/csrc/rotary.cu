@@ -12,6 +12,7 @@ namespace {
 
 constexpr int NT = 256;
 constexpr int UNROLL = 4;      // accesses a thread has in flight before it stores
+constexpr int MAX_TOKENS = 64; // per block
 
 template <typename T> __device__ __forceinline__ float to_f(T v);
 template <> __device__ __forceinline__ float to_f<float>(float v) { return v; }
@@ -29,6 +30,7 @@ struct Args {
   int64_t tokens;          // batch * num_tokens
   int tokens_per_block, heads_per_block, heads;   // heads: queries and keys together
   int turn_items, items;   // per row: accesses that rotate, and all of them
+  uint64_t items_inv, heads_inv;   // ceil(2^32 / items), ceil(2^32 / heads_per_block): exact quotients of small numbers
 };
 
 // How an access covers pairs.  MATES: V elements that are one end of V pairs, with the other ends `half` further on;
@@ -39,6 +41,7 @@ enum { MATES, INSIDE, SINGLE };
 template <typename T, int V, int MODE>
 __global__ void __launch_bounds__(NT) rotary_kernel(const Args a) {
   extern __shared__ float2 cs[];          // [tokens_per_block][half]: magnitude * {cos, sin}
+  __shared__ int64_t from[MAX_TOKENS][4];   // offsets of a token in q, k and the outputs
   const xkv_rotary_params& p = a.p;
   const int half = p.rotary_dim / 2;
   const int mate = MODE == SINGLE ? 1 : half;
@@ -47,6 +50,13 @@ __global__ void __launch_bounds__(NT) rotary_kernel(const Args a) {
   const int h0 = blockIdx.y * a.heads_per_block;
   const int nh = min(a.heads_per_block, a.heads - h0);
 
+  if (threadIdx.x < ntok) {
+    const int64_t b = (tok0 + threadIdx.x) / p.num_tokens, t = (tok0 + threadIdx.x) - b * p.num_tokens;
+    from[threadIdx.x][0] = b * p.q_sb + t * p.q_st;
+    from[threadIdx.x][1] = b * p.k_sb + t * p.k_st;
+    from[threadIdx.x][2] = b * p.qo_sb + t * p.qo_st;
+    from[threadIdx.x][3] = b * p.ko_sb + t * p.ko_st;
+  }
   for (int i = threadIdx.x; i < ntok * half; i += NT) {
     const int tl = i / half, j = i - tl * half;
     const int64_t b = (tok0 + tl) / p.num_tokens, t = (tok0 + tl) - b * p.num_tokens;
@@ -69,18 +79,16 @@ __global__ void __launch_bounds__(NT) rotary_kernel(const Args a) {
     for (int u = 0; u < UNROLL; ++u) {
       const int i = base + u * NT;
       if (i >= total) break;
-      const int row = i / a.items, c = i - row * a.items;
-      const int tl = row / nh, h = h0 + (row - tl * nh);
-      const int64_t b = (tok0 + tl) / p.num_tokens, t = (tok0 + tl) - b * p.num_tokens;
-      const bool is_q = h < p.num_heads;
+      const int row = (int)((uint32_t)i * a.items_inv >> 32), c = i - row * a.items;
+      const int tl = nh == a.heads_per_block ? (int)((uint32_t)row * a.heads_inv >> 32) : row / nh, h = h0 + (row - tl * nh);
       const T* src;
-      if (is_q) {
-        src = static_cast<const T*>(p.q) + b * p.q_sb + (int64_t)h * p.q_sh + t * p.q_st;
-        dst[u] = static_cast<T*>(p.q_out) + b * p.qo_sb + (int64_t)h * p.qo_sh + t * p.qo_st;
+      if (h < p.num_heads) {
+        src = static_cast<const T*>(p.q) + from[tl][0] + (int64_t)h * p.q_sh;
+        dst[u] = static_cast<T*>(p.q_out) + from[tl][2] + (int64_t)h * p.qo_sh;
       } else {
         const int hk = h - p.num_heads;
-        src = static_cast<const T*>(p.k) + b * p.k_sb + (int64_t)hk * p.k_sh + t * p.k_st;
-        dst[u] = static_cast<T*>(p.k_out) + b * p.ko_sb + (int64_t)hk * p.ko_sh + t * p.ko_st;
+        src = static_cast<const T*>(p.k) + from[tl][1] + (int64_t)hk * p.k_sh;
+        dst[u] = static_cast<T*>(p.k_out) + from[tl][3] + (int64_t)hk * p.ko_sh;
       }
       int off;
       if (c < a.turn_items) {
@@ -142,9 +150,18 @@ int launch(Args a, cudaStream_t st) {
   const bool few = a.tokens * per_token < (int64_t)2 * device_sm_count() * NT * UNROLL;
   a.heads_per_block = few ? (NT + a.items - 1) / a.items : a.heads;
   a.heads_per_block = a.heads_per_block < a.heads ? a.heads_per_block : a.heads;
+  a.heads_per_block = a.heads_per_block < 256 ? a.heads_per_block : 256;
   int tpb = few ? 1 : (2 * NT * UNROLL + per_token - 1) / per_token;
   const int most = 32 * 1024 / ((int)sizeof(float2) * half);
-  a.tokens_per_block = tpb < 1 ? 1 : tpb > most ? (most < 1 ? 1 : most) : tpb;
+  tpb = tpb > most ? most : tpb;
+  tpb = tpb > MAX_TOKENS ? MAX_TOKENS : tpb;
+  a.tokens_per_block = tpb < 1 ? 1 : tpb;
+  a.items_inv = (0x100000000ull + a.items - 1) / a.items;
+  a.heads_inv = (0x100000000ull + a.heads_per_block - 1) / a.heads_per_block;
+  // the quotients are exact while number * divisor < 2^32
+  if ((int64_t)a.tokens_per_block * a.heads_per_block * a.items * a.items >= 0x100000000ll ||
+      (int64_t)a.tokens_per_block * a.heads_per_block * a.heads_per_block >= 0x100000000ll)
+    return XKV_ERR_UNSUPPORTED;
   const int64_t gx = (a.tokens + a.tokens_per_block - 1) / a.tokens_per_block;
   const int gy = ceil_div(a.heads, a.heads_per_block);
   const size_t smem = (size_t)a.tokens_per_block * half * sizeof(float2);
