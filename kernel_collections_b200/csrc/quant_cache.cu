@@ -27,14 +27,128 @@ template <typename T, int V> struct alignas(sizeof(T) * V) Vec { T x[V]; };
 
 template <int CODE> __device__ __forceinline__ constexpr float largest() { return CODE == XKV_CACHE_INT8 ? 127.f : 448.f; }
 
-// y is within +-C (1 + 2^-22): a reciprocal and two products, each rounded once
-template <int CODE> __device__ __forceinline__ uint8_t encode(float y) {
-  if (CODE == XKV_CACHE_INT8) return (uint8_t)(int8_t)__float2int_rn(fminf(fmaxf(y, -127.f), 127.f));
-  return __nv_cvt_float_to_fp8(y, __NV_SATFINITE, __NV_E4M3);
+__device__ __forceinline__ float max_nan(float a, float b) {      // a NaN stays
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
 }
-template <int CODE> __device__ __forceinline__ float decode(uint8_t c) {
-  if (CODE == XKV_CACHE_INT8) return (float)(int8_t)c;
-  return __half2float(__half(__nv_cvt_fp8_to_halfraw(c, __NV_E4M3)));
+// two fp32 operations in one instruction
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  float2 r;
+  asm("{.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmul.rn.f32x2 z, x, y;\n\tmov.b64 {%0, %1}, z;}"
+      : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return r;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 r;
+  asm("{.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tadd.rn.f32x2 z, x, y;\n\tmov.b64 {%0, %1}, z;}"
+      : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return r;
+}
+__device__ __forceinline__ __half2 abs_max(__half2 a, __half2 b) { return __hmax2_nan(a, __habs2(b)); }
+__device__ __forceinline__ __nv_bfloat162 abs_max(__nv_bfloat162 a, __nv_bfloat162 b) { return __hmax2_nan(a, __habs2(b)); }
+template <typename T> struct Pair;
+template <> struct Pair<__half> {
+  using type = __half2;
+  static __device__ __forceinline__ float2 up(__half2 v) { return __half22float2(v); }
+  static __device__ __forceinline__ __half2 down(float2 v) { return __floats2half2_rn(v.x, v.y); }
+};
+template <> struct Pair<__nv_bfloat16> {
+  using type = __nv_bfloat162;
+  static __device__ __forceinline__ float2 up(__nv_bfloat162 v) { return __bfloat1622float2(v); }
+  static __device__ __forceinline__ __nv_bfloat162 down(float2 v) { return __floats2bfloat162_rn(v.x, v.y); }
+};
+
+// the largest magnitude, or NaN; 16-bit types compare in pairs (exact)
+template <typename T, int V> __device__ __forceinline__ float largest_of(const Vec<T, V>& x) {
+  if constexpr (sizeof(T) == 2 && V % 2 == 0) {
+    using P = typename Pair<T>::type;
+    const P* q = reinterpret_cast<const P*>(x.x);
+    P m = __habs2(q[0]);
+#pragma unroll
+    for (int e = 1; e < V / 2; ++e) m = abs_max(m, q[e]);
+    const float2 f = Pair<T>::up(m);
+    return max_nan(f.x, f.y);
+  } else {
+    float m = 0.f;
+#pragma unroll
+    for (int e = 0; e < V; ++e) m = max_nan(m, fabsf(to_f(x.x[e])));
+    return m;
+  }
+}
+template <typename T, int V> __device__ __forceinline__ float2 two_of(const Vec<T, V>& x, int e) {
+  if constexpr (sizeof(T) == 2) return Pair<T>::up(reinterpret_cast<const typename Pair<T>::type*>(x.x)[e / 2]);
+  else return make_float2(x.x[e], x.x[e + 1]);
+}
+
+// codes of x * per.  |x * per| is at most C (1 + 2^-22) (a reciprocal and two products, each rounded once), which still
+// rounds to C: nothing to clamp.  int8: adding 1.5 * 2^23 rounds to the nearest integer, ties to even, and leaves it in the
+// low byte.
+template <typename T, int CODE, int V> __device__ __forceinline__ Vec<uint8_t, V> encode(const Vec<T, V>& x, float per) {
+  Vec<uint8_t, V> c;
+  if constexpr (V % 4 == 0) {
+    uint32_t* out = reinterpret_cast<uint32_t*>(c.x);
+#pragma unroll
+    for (int e = 0; e < V; e += 4) {
+      float2 a = two_of(x, e), b = two_of(x, e + 2);
+      if (CODE == XKV_CACHE_INT8) {
+        // the product is rounded before the sum: paired instructions were seen to become one fused multiply-add here
+        a.x = __fadd_rn(__fmul_rn(a.x, per), 12582912.f);
+        a.y = __fadd_rn(__fmul_rn(a.y, per), 12582912.f);
+        b.x = __fadd_rn(__fmul_rn(b.x, per), 12582912.f);
+        b.y = __fadd_rn(__fmul_rn(b.y, per), 12582912.f);
+        out[e / 4] = __byte_perm(__byte_perm(__float_as_uint(a.x), __float_as_uint(a.y), 0x0040u),
+                                 __byte_perm(__float_as_uint(b.x), __float_as_uint(b.y), 0x0040u), 0x5410u);
+      } else {
+        a = mul2(a, make_float2(per, per));
+        b = mul2(b, make_float2(per, per));
+        out[e / 4] = (uint32_t)__nv_cvt_float2_to_fp8x2(a, __NV_SATFINITE, __NV_E4M3) |
+                     (uint32_t)__nv_cvt_float2_to_fp8x2(b, __NV_SATFINITE, __NV_E4M3) << 16;
+      }
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+      const float y = __fmul_rn(to_f(x.x[e]), per);
+      c.x[e] = CODE == XKV_CACHE_INT8 ? (uint8_t)__float_as_uint(__fadd_rn(y, 12582912.f)) : __nv_cvt_float_to_fp8(y, __NV_SATFINITE, __NV_E4M3);
+    }
+  }
+  return c;
+}
+// code * scale.  int8: a code with its sign bit flipped under the upper bytes of 2^23 is the float 2^23 + 128 + code.
+template <typename T, int CODE, int V> __device__ __forceinline__ Vec<T, V> decode(const Vec<uint8_t, V>& c, float scale) {
+  Vec<T, V> x;
+  if constexpr (V % 4 == 0) {
+#pragma unroll
+    for (int e = 0; e < V; e += 4) {
+      const uint32_t w = reinterpret_cast<const uint32_t*>(c.x)[e / 4];
+      float2 a, b;
+      if (CODE == XKV_CACHE_INT8) {
+        const uint32_t y = w ^ 0x80808080u;
+        const float2 off = make_float2(-8388736.f, -8388736.f);
+        a = add2(make_float2(__uint_as_float(__byte_perm(y, 0x4b000000u, 0x7440u)), __uint_as_float(__byte_perm(y, 0x4b000000u, 0x7441u))), off);
+        b = add2(make_float2(__uint_as_float(__byte_perm(y, 0x4b000000u, 0x7442u)), __uint_as_float(__byte_perm(y, 0x4b000000u, 0x7443u))), off);
+      } else {
+        a = __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w & 0xffffu), __NV_E4M3)));
+        b = __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w >> 16), __NV_E4M3)));
+      }
+      a = mul2(a, make_float2(scale, scale));
+      b = mul2(b, make_float2(scale, scale));
+      if constexpr (sizeof(T) == 2) {
+        reinterpret_cast<typename Pair<T>::type*>(x.x)[e / 2] = Pair<T>::down(a);
+        reinterpret_cast<typename Pair<T>::type*>(x.x)[e / 2 + 1] = Pair<T>::down(b);
+      } else {
+        x.x[e] = a.x; x.x[e + 1] = a.y; x.x[e + 2] = b.x; x.x[e + 3] = b.y;
+      }
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+      const float y = CODE == XKV_CACHE_INT8 ? (float)(int8_t)c.x[e] : __half2float(__half(__nv_cvt_fp8_to_halfraw(c.x[e], __NV_E4M3)));
+      x.x[e] = from_f<T>(y * scale);
+    }
+  }
+  return x;
 }
 
 // A block works on one (sequence, KV head) of the keys or of the values: grid (2 x token chunks, KV heads, sequences).
@@ -85,23 +199,12 @@ __global__ void __launch_bounds__(NT) append_kernel(const xkv_cache_params p, in
     const int64_t at = w.start + t;
     const bool live = t < w.tokens && at >= 0 && at < p.capacity;
     float top = 0.f;
-    bool odd = false;       // an infinity or a NaN
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int d = (i * lanes + w.lane) * V;
-      if (t < w.tokens && d < p.head_dim) {
-#pragma unroll
-        for (int e = 0; e < V; ++e) {
-          const float m = fabsf(to_f(x[u][i].x[e]));
-          odd |= !(m <= 3.402823466e38f);
-          top = fmaxf(top, m);
-        }
-      }
-    }
-    if (odd) top = CUDART_INF_F;       // fmaxf passes a NaN over, an infinity survives it
-    for (int o = lanes >> 1; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    for (int i = 0; i < NV; ++i)
+      if (t < w.tokens && (i * lanes + w.lane) * V < p.head_dim) top = max_nan(top, largest_of(x[u][i]));
+    for (int o = lanes >> 1; o; o >>= 1) top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, o));
     if (!live) continue;
-    const bool finite = top < CUDART_INF_F;
+    const bool finite = top < CUDART_INF_F;      // not an infinity, not a NaN
     float scale = __fmul_rn(top, 1.0f / largest<CODE>());
     float per = 0.f;
     if (!finite) scale = CUDART_NAN_F;
@@ -111,9 +214,8 @@ __global__ void __launch_bounds__(NT) append_kernel(const xkv_cache_params p, in
     for (int i = 0; i < NV; ++i) {
       const int d = (i * lanes + w.lane) * V;
       if (d < p.head_dim) {
-        Vec<uint8_t, V> c;
-#pragma unroll
-        for (int e = 0; e < V; ++e) c.x[e] = finite ? encode<CODE>(to_f(x[u][i].x[e]) * per) : 0;
+        Vec<uint8_t, V> c = {};
+        if (finite) c = encode<T, CODE, V>(x[u][i], per);
         *reinterpret_cast<Vec<uint8_t, V>*>(codes + at * sl + d) = c;
       }
     }
@@ -149,11 +251,8 @@ __global__ void __launch_bounds__(NT) read_kernel(const xkv_cache_params p, int 
     for (int u = 0; u < U; ++u) {
       const int t = t0 + u * w.groups;
       if (t >= w.tokens) break;
-      const int64_t at = w.start + t;
-      const bool live = at >= 0 && at < p.capacity;
-      Vec<T, V> x;
-#pragma unroll
-      for (int e = 0; e < V; ++e) x.x[e] = from_f<T>(live ? decode<CODE>(c[u].x[e]) * scale[u] : 0.f);
+      // outside the cache: zeros (code 0, scale 0)
+      const Vec<T, V> x = decode<T, CODE, V>(c[u], scale[u]);
       *reinterpret_cast<Vec<T, V>*>(dst + t * st + d) = x;
     }
   }
