@@ -19,8 +19,8 @@
 //    queries subtract it; so do the values, whose sums run over thousands of tokens.)
 //  * Scales never touch the codes: the key scale multiplies the score, the value scale the weight.
 //  * fp16 ranges: a query row is multiplied by a power of two that brings its largest element to 2^14..2^15, and divided
-//    out of the scores in fp32: elements below 2^-28 of the largest lose bits, others none.  Weights carry the factor 2^12
-//    (it cancels in O / l) so that those down to 2^-26 of the largest keep all 11 bits, and the value scales are taken
+//    out of the scores in fp32: elements below 2^-28 of the largest lose bits, others none.  Weights carry the factor 2^6
+//    (it cancels in O / l) so that those down to 2^-20 of the largest keep all 11 bits, and the value scales are taken
 //    relative to a power of two above the largest seen.
 //  * fp32 queries: Q and P in two fp16 terms each (22 bits), two MMAs instead of one.
 #include "tree_common.cuh"
@@ -131,7 +131,7 @@ __global__ void __launch_bounds__(NT, 1) stream_kernel(const Args a) {
   constexpr int E = WIDE ? 2 : 1;                  // tokens of every 8 that a thread scores, for each of its rows
   constexpr int QV = WIDE ? 1 : 2;                 // k-steps per 16 bytes of query operand
   // weights are 2^(score - reference + LIFT); the reference follows the maximum when it is passed by more than SLACK
-  constexpr float LIFT = std::is_same<M, __half>::value ? 12.f : 0.f, SLACK = std::is_same<M, __half>::value ? 3.f : 8.f;
+  constexpr float LIFT = std::is_same<M, __half>::value ? 6.f : 0.f, SLACK = std::is_same<M, __half>::value ? 9.f : 32.f;
   extern __shared__ __align__(128) uint8_t smem[];
   const xkv_tree_params& p = a.p;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;

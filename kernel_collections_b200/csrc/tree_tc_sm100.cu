@@ -10,10 +10,11 @@
 // same rows and take alternate tiles, each with its own O; the two are joined at the end.  An "item" is one tile for one
 // group; S of item j + 2 is issued right after P.V of item j, into the same columns (MMAs run in order).
 //   warps 0-7  softmax          warp 8  MMA issuer (one thread) and tensor-memory allocation
-//   16-bit caches: warp 9 brings tiles by TMA.  8-bit caches: warps 9-12 load codes into registers one tile ahead, widen
+//   16-bit caches: warp 9 brings tiles by TMA.  8-bit caches: warps 12-15 load codes into registers one tile ahead, widen
 //   them to fp16 (exact) and store them in the layout that TMA would have made; scales go to the softmax threads.
-// The softmax reads S twice, for the maximum and for the weights: tensor memory gives it to the registers faster than the
-// exponentials need it, and so 64 columns are in registers at a time instead of 128.  Number ranges (query scaling, LIFT, value scales relative to a power of two) are those of
+// The softmax takes one pass over S as long as no row's reference has to move (lazily, see SLACK below): weights are
+// taken against the old reference while the new maximum is formed, kept in registers, and taken again in the rare tile that
+// moves a reference or holds drafted tokens.  Number ranges (query scaling, LIFT, value scales relative to a power of two) are those of
 // tree_stream_sm100.cu.  P is rounded to the 16-bit type of the product and l sums the rounded values.
 // All waits are bounded; a group that gives up raises the abort flag, which ends the others' waits.
 #include "tree_common.cuh"
@@ -30,7 +31,9 @@ constexpr int STAGES = 2;                   // of K and of V each
 constexpr int BOX = TK * 128;               // bytes of [128 tokens or rows] x 64 dims
 constexpr int MAX_T = 256;                  // drafted tokens whose mask fits its place
 
-template <int CODE> constexpr int threads() { return CODE == XKV_CACHE_DENSE ? 320 : 416; }
+// 16-bit caches: three warps per scheduler, 168 registers each.  8-bit: four, 128 at launch, moved from the issuer's and the
+// wideners' warpgroups to the softmax (2 x 168 + 2 x 88 = 4 x 128).
+template <int CODE> constexpr int threads() { return CODE == XKV_CACHE_DENSE ? 320 : 512; }
 
 template <int D, int MB>
 struct Smem {
@@ -75,6 +78,13 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
 template <typename T> __device__ __forceinline__ float to_float(T v) { return TypeTraits<T>::to_f(v); }
 template <typename T> __device__ __forceinline__ T from_float(float v) { return TypeTraits<T>::from_f(v); }
 
+// one lane of the warp, the same one every time
+__device__ __forceinline__ bool elect() {
+  uint32_t one;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(one));
+  return one != 0;
+}
+
 // bytes 0, 1 of x (high = 0) or 2, 3 as two halves; int8 with its sign bits flipped beforehand
 template <int CODE> __device__ __forceinline__ uint32_t widen(uint32_t x, int high) {
   if (CODE == XKV_CACHE_INT8) {
@@ -95,7 +105,8 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
   using M = typename std::conditional<Q8, __half, T>::type;
   using S = Smem<D, MB>;
   // weights are 2^(score - reference + LIFT); the reference follows the maximum when it is passed by more than SLACK
-  constexpr float LIFT = std::is_same<M, __half>::value ? 12.f : 0.f, SLACK = std::is_same<M, __half>::value ? 3.f : 8.f;
+  // (fp16: below 2^15 always, and all 11 bits down to 2^-20 of the reference; bf16 has the range of fp32)
+  constexpr float LIFT = std::is_same<M, __half>::value ? 6.f : 0.f, SLACK = std::is_same<M, __half>::value ? 9.f : 32.f;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw = smem_u32(smem_raw);
   const uint32_t base = (raw + 1023u) & ~1023u;
@@ -118,14 +129,14 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; ++s) {
-      mbar_init(bar_kfull(s), Q8 ? 128 : 1);
-      mbar_init(bar_vfull(s), Q8 ? 128 : 1);
+      mbar_init(bar_kfull(s), Q8 ? 4 : 1);               // one arrival per warp
+      mbar_init(bar_vfull(s), Q8 ? 4 : 1);
       mbar_init(bar_kempty(s), 1);
       mbar_init(bar_vempty(s), 1);
     }
-    for (int w = 0; w < 2; ++w) { mbar_init(bar_s(w), 1); mbar_init(bar_p(w), 128); }
-    mbar_init(bar_q, 256);
-    mbar_init(bar_end, 256);
+    for (int w = 0; w < 2; ++w) { mbar_init(bar_s(w), 1); mbar_init(bar_p(w), 4); }
+    mbar_init(bar_q, 8);
+    mbar_init(bar_end, 8);
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -137,7 +148,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = *tmem_slot;        // columns: S / P of the groups at 0 and 128, O at 256 and 384
+  const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);        // columns: S / P of the groups at 0 and 128, O at 256 and 384
   asm volatile("griddepcontrol.launch_dependents;");
   if (blockIdx.x == 0 && threadIdx.x < 8) a.status[threadIdx.x] = 0;      // a wait takes far longer than this to give up
 
@@ -145,6 +156,10 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
   Piece pc = {};
   auto tiles_of = [&](const Piece& x, int len) { return max(0, min(x.end, (len + TK - 1) / TK) - x.begin); };
 
+  if constexpr (Q8) {                       // whole warpgroups: 0 1 | 2 (the issuer's) 3 (the wideners')
+    if (warp < 8) asm volatile("setmaxnreg.inc.sync.aligned.u32 168;");
+    else asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+  }
   if (warp < 8) {
     // ================================ softmax ================================================================
     const int w = warp >> 2, r = threadIdx.x & 127;         // group; row of its 128 = tensor-memory lane
@@ -163,8 +178,12 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
       if (lane == 0) report(a.status, XKV_ERR_TIMEOUT, role, pc.b, pc.h, pc.begin);
       return false;
     };
+    auto arrive = [&](uint32_t bar) {       // for the warp, once all its lanes are there
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar);
+    };
     auto meet = [&]() {
-      mbar_arrive(bar_end);
+      arrive(bar_end);
       const bool good = wait(bar_end, end_phase, 53);
       end_phase ^= 1u;
       return good;
@@ -185,7 +204,9 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
         const bool wide = reinterpret_cast<uintptr_t>(p.q) % (PER * 2) == 0 && p.q_sb % PER == 0 && p.q_sh % PER == 0 && p.q_st % PER == 0;
         struct alignas(PER * 2) Few { T x[PER]; };
         const int first_row = (pc.rb * MB + blk) * 128 + (warp & 3) * 32;
-        for (int i0 = 0; i0 < 32; i0 += AHEAD) {
+        int qh = first_row / T_, qt = first_row - qh * T_;
+        const T* src = static_cast<const T*>(p.q) + (int64_t)pc.b * p.q_sb + (int64_t)(pc.h * G + qh) * p.q_sh + (int64_t)qt * p.q_st + lane * PER;
+        for (int i0 = 0; i0 < 32 && busy; i0 += AHEAD) {
           Few q[AHEAD];
 #pragma unroll
           for (int i = 0; i < AHEAD; ++i) {
@@ -193,12 +214,15 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
 #pragma unroll
             for (int e = 0; e < PER; ++e) q[i].x[e] = from_float<T>(0.f);
             if (qr < a.rows) {
-              const T* src = static_cast<const T*>(p.q) + (int64_t)pc.b * p.q_sb + (int64_t)(pc.h * G + qr / T_) * p.q_sh +
-                             (int64_t)(qr % T_) * p.q_st + lane * PER;
               if (wide) q[i] = *reinterpret_cast<const Few*>(src);
               else
 #pragma unroll
                 for (int e = 0; e < PER; ++e) q[i].x[e] = src[e];
+              src += p.q_st;
+              if (++qt == T_) {
+                qt = 0;
+                src += p.q_sh - T_ * p.q_st;
+              }
             }
           }
 #pragma unroll
@@ -238,7 +262,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
         }
         if (threadIdx.x < MAX_T / 32) bad_s[threadIdx.x] = 0;
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        mbar_arrive(bar_q);
+        arrive(bar_q);
         if (!(ok = wait(bar_q, q_phase, 50))) break;
         q_phase ^= 1u;
       }
@@ -264,60 +288,104 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
           return __funnelshift_r(word(k), word(k + 1), u0 & 31);
         };
         if (busy) {
-          constexpr int W = Q8 ? 32 : 64;                     // columns in registers at a time
           const float2 rs2 = make_float2(row_scale, row_scale);
-          // columns c .. c + W - 1 as scores (without row_scale)
-          auto scores = [&](int c, float2 (&x)[W / 2]) {
-            uint32_t v[W / 32][32];
-#pragma unroll
-            for (int k = 0; k < W / 32; ++k) tmem_ld32(t_s + c + 32 * k, v[k]);
+          // columns c .. c + 31 as scores (without row_scale)
+          auto scores = [&](int c, float2 (&x)[16]) {
+            uint32_t v[32];
+            tmem_ld32(t_s + c, v);
             tmem_wait_ld();
 #pragma unroll
-            for (int k = 0; k < W / 2; ++k) {
-              x[k] = make_float2(__uint_as_float(v[k >> 4][2 * (k & 15)]), __uint_as_float(v[k >> 4][2 * (k & 15) + 1]));
-              if (Q8) x[k] = mul2(x[k], *reinterpret_cast<const float2*>(ks + c + 2 * k));
+            for (int k = 0; k < 16; k += 2) {
+              x[k] = make_float2(__uint_as_float(v[2 * k]), __uint_as_float(v[2 * k + 1]));
+              x[k + 1] = make_float2(__uint_as_float(v[2 * k + 2]), __uint_as_float(v[2 * k + 3]));
+              if (Q8) {
+                const float4 f = *reinterpret_cast<const float4*>(ks + c + 2 * k);
+                x[k] = mul2(x[k], make_float2(f.x, f.y));
+                x[k + 1] = mul2(x[k + 1], make_float2(f.z, f.w));
+              }
             }
           };
-          uint32_t bits[TK / 32];
-          float mx = -CUDART_INF_F, top = plain ? tile_top : 0.f;
+          float b1, inv = 1.f;
+          auto settle = [&]() {                               // what follows from ref and unit
+            b1 = ref == -CUDART_INF_F ? 0.f : LIFT - ref;
+            if (Q8) inv = unit > 0.f ? 1.f / unit : 0.f;
+          };
+          settle();
+          // their weights against the reference, packed, and the sum of them
+          auto weights = [&](int c, const float2 (&x)[16], uint32_t bits, float2& sum, uint32_t* pk) {
 #pragma unroll
-          for (int c = 0; c < TK; c += W) {
-            float2 x[W / 2];
-            scores(c, x);
-            if (plain) {
+            for (int k = 0; k < 16; ++k) {
+              const float2 y = fma2(x[k], rs2, make_float2(b1, b1));
+              float2 e = make_float2(ex2(y.x), ex2(y.y));
+              if (bits != 0xffffffffu) {                      // what a hidden token holds may be anything
+                if (!(bits >> (2 * k) & 1u)) e.x = 0.f;
+                if (!(bits >> (2 * k + 1) & 1u)) e.y = 0.f;
+              }
+              if (Q8) {
+                sum = add2(sum, e);
+                const float2 v = *reinterpret_cast<const float2*>(vs + c + 2 * k);
+                e = mul2(e, mul2(v, make_float2(inv, inv)));
+                if (bits != 0xffffffffu) {
+                  if (!(bits >> (2 * k) & 1u)) e.x = 0.f;
+                  if (!(bits >> (2 * k + 1) & 1u)) e.y = 0.f;
+                }
+              }
+              pk[k] = TypeTraits<M>::pack2(e.x, e.y);
+              if (!Q8) sum = add2(sum, TypeTraits<M>::unpack2(pk[k]));
+            }
+          };
+          float mx = -CUDART_INF_F;
+          bool done = false, known = false;                   // the row's maximum is known
+          if (__all_sync(0xffffffffu, plain && tile_top <= unit && ref > -CUDART_INF_F)) {
+            uint32_t pk[2][32];
+            float2 sum = l;
 #pragma unroll
-              for (int k = 0; k < W / 32; ++k) bits[c / 32 + k] = 0xffffffffu;
+            for (int c = 0; c < TK; c += 32) {
+              float2 x[16];
+              scores(c, x);
 #pragma unroll
-              for (int k = 0; k < W / 2; ++k) mx = fmaxf(mx, fmaxf(x[k].x, x[k].y));
-            } else {
+              for (int k = 0; k < 16; ++k) mx = fmaxf(mx, fmaxf(x[k].x, x[k].y));
+              weights(c, x, 0xffffffffu, sum, pk[c / 64] + (c & 32) / 2);
+            }
+            done = __all_sync(0xffffffffu, mx * row_scale <= ref + SLACK);
+            known = true;
+            if (done) {
+              l = sum;
+              tmem_st32(t_s, pk[0]);
+              tmem_st32(t_s + 32, pk[1]);
+            }
+          }
+          if (!done) {                                        // S is still there: P has not been stored
+            float top = plain ? tile_top : 0.f;
+#pragma unroll 1
+            for (int c = 0; c < TK && !known; c += 32) {
+              float2 x[16];
+              scores(c, x);
+              const uint32_t bits = plain ? 0xffffffffu : seen(c);
 #pragma unroll
-              for (int k = 0; k < W / 2; ++k) {
-                if (k % 16 == 0) bits[c / 32 + k / 16] = seen(c + 2 * k);
-                const uint32_t two = bits[c / 32 + k / 16] >> (2 * k & 31);
+              for (int k = 0; k < 16; ++k) {
+                const uint32_t two = bits >> (2 * k);
                 if (two & 1u) mx = fmaxf(mx, x[k].x);
                 if (two & 2u) mx = fmaxf(mx, x[k].y);
-                if (Q8) {
+                if (Q8 && !plain) {
                   const float2 v = *reinterpret_cast<const float2*>(vs + c + 2 * k);
                   if ((two & 1u) && fabsf(v.x) < CUDART_INF_F) top = fmaxf(top, fabsf(v.x));
                   if ((two & 2u) && fabsf(v.y) < CUDART_INF_F) top = fmaxf(top, fabsf(v.y));
                 }
               }
             }
-          }
-          mx *= row_scale;
-          const bool up_ref = mx > ref + SLACK, up_unit = Q8 && top > unit;       // by the row's own: rows stay independent
-          if (__any_sync(0xffffffffu, up_ref || up_unit)) {
-            const float to = up_ref ? mx : ref;
+            mx *= row_scale;
+            const float to = mx > ref + SLACK ? mx : ref;     // by the row's own scores: rows stay independent
             float f = to == -CUDART_INF_F ? 1.f : exp2f(ref - to);
             ref = to;
             l = mul2(l, make_float2(f, f));
-            if (up_unit) {
+            if (Q8 && top > unit) {
               const uint32_t e = min((__float_as_uint(top) >> 23) + 1u, 254u);
               const float to_v = __uint_as_float(e << 23);
               f *= unit / to_v;
               unit = to_v;
             }
-            if (items > 0) {                                  // S of this item is behind P.V of the last one
+            if (items > 0 && __any_sync(0xffffffffu, f != 1.f)) {      // S of this item is behind P.V of the last one
 #pragma unroll 1
               for (int c = 0; c < D; c += 32) {
                 uint32_t v[32];
@@ -328,37 +396,15 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
                 tmem_st32(t_o + c, v);
               }
             }
-          }
-          const float b1 = ref == -CUDART_INF_F ? 0.f : LIFT - ref;
-          const float inv = Q8 ? (unit > 0.f ? 1.f / unit : 0.f) : 1.f;
-#pragma unroll
-          for (int c = 0; c < TK; c += W) {                   // P of W columns takes W / 2, behind what is still to be read
-            float2 x[W / 2];
-            scores(c, x);
-            uint32_t pk[W / 2];
-#pragma unroll
-            for (int k = 0; k < W / 2; ++k) {
-              const uint32_t two = bits[c / 32 + k / 16] >> (2 * k & 31);
-              const float2 y = fma2(x[k], rs2, make_float2(b1, b1));
-              float2 e = make_float2(ex2(y.x), ex2(y.y));
-              if (Q8) {
-                const float2 v = mul2(*reinterpret_cast<const float2*>(vs + c + 2 * k), make_float2(inv, inv));
-                if (!plain) {                                 // what a hidden token holds, scales too, may be anything
-                  if (!(two & 1u)) e.x = 0.f;
-                  if (!(two & 2u)) e.y = 0.f;
-                }
-                l = add2(l, e);
-                e = mul2(e, v);
-              }
-              if (!plain) {
-                if (!(two & 1u)) e.x = 0.f;
-                if (!(two & 2u)) e.y = 0.f;
-              }
-              pk[k] = TypeTraits<M>::pack2(e.x, e.y);
-              if (!Q8) l = add2(l, TypeTraits<M>::unpack2(pk[k]));
+            settle();
+#pragma unroll 1
+            for (int c = 0; c < TK; c += 32) {                // P of 32 columns takes 16, behind what is still to be read
+              float2 x[16];
+              uint32_t pk[16];
+              scores(c, x);
+              weights(c, x, plain ? 0xffffffffu : seen(c), l, pk);
+              tmem_st16(t_s + c / 2, pk);
             }
-            if constexpr (Q8) tmem_st16(t_s + c / 2, pk);
-            else tmem_st32(t_s + c / 2, pk);
           }
           tmem_wait_st();
         }
@@ -388,7 +434,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
           asm volatile("fence.proxy.async.shared::cta;" ::: "memory");      // before the MMA reads the tile
         }
         tc_fence_before();
-        mbar_arrive(bar_p(w));
+        arrive(bar_p(w));
       }
       if (!ok) break;
       tiles_seen += ntiles;
@@ -475,7 +521,11 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
     }
   } else if (warp == 8) {
     // ================================ MMA issuer =============================================================
-    if (lane == 0) {
+    {
+      // The whole warp walks the loop and one lane issues: operands that are the same in all lanes stay in uniform
+      // registers, where the MMA wants them.  (One thread alone moved them there for every MMA and spent twice the time
+      // of the MMA on it.)
+      const bool lead = elect();
       constexpr uint32_t F = TypeTraits<M>::kFmt;
       constexpr uint32_t id_s = (1u << 4) | (F << 7) | (F << 10) | ((TK >> 3) << 17) | ((128u >> 4) << 24);
       constexpr uint32_t id_o = (1u << 4) | (F << 7) | (F << 10) | (1u << 16) | (((uint32_t)D >> 3) << 17) | ((128u >> 4) << 24);
@@ -484,14 +534,13 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
       int seen = 0;
       bool ok = true;
       auto waits = [&](uint32_t bar, uint32_t parity, int role) {
-        if (mbar_wait(bar, parity, abort_flag)) return true;
-        report(a.status, XKV_ERR_TIMEOUT, role, pc.b, pc.h, pc.begin);
+        if (__all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag))) return true;
+        if (lane == 0) report(a.status, XKV_ERR_TIMEOUT, role, pc.b, pc.h, pc.begin);
         return false;
       };
-      // the walk's collectives are behind us: from here on this thread steps alone
       while (ok && next_piece(a, walk, pc)) {
         const Span sp = span_of(p, pc.b);
-        const int ntiles = tiles_of(pc, sp.len), items = ntiles * MB;
+        const int items = __shfl_sync(0xffffffffu, tiles_of(pc, sp.len), 0) * MB;
         if (!(ok = waits(bar_q, q_phase, 60))) break;
         q_phase ^= 1u;
         tc_fence_after();
@@ -500,12 +549,15 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
           if (!waits(bar_kfull(stage), (uint32_t)(tile / STAGES) & 1u, 61)) return false;
           tc_fence_after();
           const uint64_t q = desc_advance(dq, MB == 2 ? (uint32_t)(w * S::TILE) : 0u), k = desc_advance(dk, (uint32_t)(stage * S::TILE));
+          const uint32_t d = tmem + (uint32_t)w * 128u;
+          if (lead) {
 #pragma unroll
-          for (int s = 0; s < D / 16; ++s)
-            tc_mma(tmem + (uint32_t)w * 128u, desc_advance(q, (s >> 2) * BOX + (s & 3) * 32), desc_advance(k, (s >> 2) * BOX + (s & 3) * 32),
-                   id_s, s ? 1u : 0u);
-          tc_commit(bar_s(w));
-          if (MB == 1 || w == 1) tc_commit(bar_kempty(stage));
+            for (int s = 0; s < D / 16; ++s)
+              tc_mma(d, desc_advance(q, (s >> 2) * BOX + (s & 3) * 32), desc_advance(k, (s >> 2) * BOX + (s & 3) * 32), id_s, s ? 1u : 0u);
+            tc_commit(bar_s(w));
+            if (MB == 1 || w == 1) tc_commit(bar_kempty(stage));
+          }
+          __syncwarp();
           return true;
         };
         for (int j = 0; j < 2 && j < items; ++j)
@@ -517,15 +569,18 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
           if (!(ok = waits(bar_vfull(stage), (uint32_t)(tile / STAGES) & 1u, 63))) break;
           tc_fence_after();
           const uint64_t v = desc_advance(dv, (uint32_t)(stage * S::TILE));
+          const uint32_t o = tmem + 256u + (uint32_t)w * 128u, pt = tmem + (uint32_t)w * 128u, first = j < 2 ? 0u : 1u;
+          if (lead) {
+            tc_mma_ts(o, pt, v, id_o, first);
 #pragma unroll
-          for (int s = 0; s < TK / 16; ++s)
-            tc_mma_ts(tmem + 256u + (uint32_t)w * 128u, tmem + (uint32_t)w * 128u + s * 8, desc_advance(v, s * 2048), id_o,
-                      (j < 2 && s == 0) ? 0u : 1u);
-          if (MB == 1 || w == 1) tc_commit(bar_vempty(stage));
+            for (int s = 1; s < TK / 16; ++s) tc_mma_ts(o, pt + s * 8, desc_advance(v, s * 2048), id_o, 1u);
+            if (MB == 1 || w == 1) tc_commit(bar_vempty(stage));
+            if (j + 2 >= items) tc_commit(bar_s(w));        // the group's last P.V
+          }
+          __syncwarp();
           if (j + 2 < items) ok = scores(j + 2);
-          else tc_commit(bar_s(w));                         // the group's last P.V
         }
-        seen += ntiles;
+        seen += items / MB;
       }
     }
     __syncwarp();
@@ -556,10 +611,10 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
       }
     }
     __syncwarp();
-  } else {
+  } else if (warp >= 12) {
     // ================================ codes widened into tiles ===============================================
     constexpr int CH = D / 16, RPI = 32 / CH, N = 32 / RPI;      // 16-byte pieces of a row; rows per access of the warp; accesses
-    const int c4 = warp - 9, r0 = lane / CH, c = lane % CH;      // this warp's 32 tokens of a tile start at 32 c4
+    const int c4 = warp - 12, r0 = lane / CH, c = lane % CH;      // this warp's 32 tokens of a tile start at 32 c4
     int seen = 0;
     bool ok = true;
     uint4 kr[N], vr[N];
@@ -619,7 +674,8 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
         if (!(ok = wait(bar_kempty(stage), parity, 70))) break;
         store(kr, S::K + stage * S::TILE);
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        mbar_arrive(bar_kfull(stage));
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar_kfull(stage));
         const float k_scale = ksr;
         if (i + 1 < ntiles) load_k(i + 1);
         if (!(ok = wait(bar_vempty(stage), parity, 71))) break;
@@ -650,7 +706,8 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
         const uint32_t top = __reduce_max_sync(0xffffffffu, mag < 0x7f800000u ? mag : 0u);
         if (lane == 0) ks[2 * TK + c4] = __uint_as_float(top);
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        mbar_arrive(bar_vfull(stage));
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar_vfull(stage));
         if (i + 1 < ntiles) load_v(i + 1);
       }
     }
