@@ -10,7 +10,7 @@
 // same rows and take alternate tiles, each with its own O; the two are joined at the end.  An "item" is one tile for one
 // group; S of item j + 2 is issued right after P.V of item j, into the same columns (MMAs run in order).
 //   warps 0-7  softmax          warp 8  MMA issuer (one thread) and tensor-memory allocation
-//   16-bit caches: warp 9 brings tiles by TMA.  8-bit caches: warps 12-15 load codes into registers one tile ahead, widen
+//   16-bit caches: warp 9 brings tiles by TMA.  8-bit caches: warps 12-19 load codes into registers one tile ahead, widen
 //   them to fp16 (exact) and store them in the layout that TMA would have made; scales go to the softmax threads.
 // The softmax takes one pass over S as long as no row's reference has to move (lazily, see SLACK below): weights are
 // taken against the old reference while the new maximum is formed, kept in registers, and taken again in the rare tile that
@@ -31,9 +31,10 @@ constexpr int STAGES = 2;                   // of K and of V each
 constexpr int BOX = TK * 128;               // bytes of [128 tokens or rows] x 64 dims
 constexpr int MAX_T = 256;                  // drafted tokens whose mask fits its place
 
-// 16-bit caches: three warps per scheduler, 168 registers each.  8-bit: four, 128 at launch, moved from the issuer's and the
-// wideners' warpgroups to the softmax (2 x 168 + 2 x 88 = 4 x 128).
-template <int CODE> constexpr int threads() { return CODE == XKV_CACHE_DENSE ? 320 : 512; }
+// 16-bit caches: three warps per scheduler, 168 registers each.  8-bit: five, 96 at launch, moved from the issuer's and the
+// wideners' warpgroups to the softmax (2 x 144 + 3 x 64 = 5 x 96).
+constexpr int WIDENERS = 8;                 // warps
+template <int CODE> constexpr int threads() { return CODE == XKV_CACHE_DENSE ? 320 : 640; }
 
 template <int D, int MB>
 struct Smem {
@@ -42,8 +43,8 @@ struct Smem {
   static constexpr int Q = 0;                                   // two row blocks (the second also takes part in the join)
   static constexpr int K = Q + 2 * TILE;
   static constexpr int V = K + STAGES * TILE;
-  static constexpr int SCALES = V + STAGES * TILE;              // [stage]{key scales, value scales}[128], [stage][4] largest
-  static constexpr int MASK = SCALES + STAGES * (2 * TK + 4) * 4;   // [token][words]
+  static constexpr int SCALES = V + STAGES * TILE;              // [stage]{key scales, value scales}[128], [stage] the wideners' largest
+  static constexpr int MASK = SCALES + STAGES * (2 * TK + WIDENERS) * 4;   // [token][words]
   static constexpr int BAD = MASK + MAX_T * (MAX_T / 32) * 4;   // drafted tokens with values that are not finite
   static constexpr int ML = BAD + MAX_T / 32 * 4;               // [128] of the second group, MB == 1
   static constexpr int BAR = ML + TK * 8;
@@ -129,8 +130,8 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; ++s) {
-      mbar_init(bar_kfull(s), Q8 ? 4 : 1);               // one arrival per warp
-      mbar_init(bar_vfull(s), Q8 ? 4 : 1);
+      mbar_init(bar_kfull(s), Q8 ? WIDENERS : 1);        // one arrival per warp
+      mbar_init(bar_vfull(s), Q8 ? WIDENERS : 1);
       mbar_init(bar_kempty(s), 1);
       mbar_init(bar_vempty(s), 1);
     }
@@ -156,9 +157,9 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
   Piece pc = {};
   auto tiles_of = [&](const Piece& x, int len) { return max(0, min(x.end, (len + TK - 1) / TK) - x.begin); };
 
-  if constexpr (Q8) {                       // whole warpgroups: 0 1 | 2 (the issuer's) 3 (the wideners')
-    if (warp < 8) asm volatile("setmaxnreg.inc.sync.aligned.u32 168;");
-    else asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+  if constexpr (Q8) {                       // whole warpgroups: 0 1 | 2 (the issuer's) 3 4 (the wideners')
+    if (warp < 8) asm volatile("setmaxnreg.inc.sync.aligned.u32 144;");
+    else asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
   }
   if (warp < 8) {
     // ================================ softmax ================================================================
@@ -273,14 +274,17 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
         const int t0 = (pc.begin + i) * TK;
         const int stage = (tiles_seen + i) % STAGES;
         const uint32_t v_parity = (uint32_t)((tiles_seen + i) / STAGES) & 1u;
-        const float* ks = reinterpret_cast<const float*>(sm + S::SCALES + stage * (2 * TK + 4) * 4);
+        const float* ks = reinterpret_cast<const float*>(sm + S::SCALES + stage * (2 * TK + WIDENERS) * 4);
         const float* vs = ks + TK;
         if (Q8 && !(ok = wait(bar_vfull(stage), v_parity, 51))) break;       // the scales come with the values
         if (!(ok = wait(bar_s(w), s_phase, 52))) break;
         s_phase ^= 1u;
         tc_fence_after();
         const bool plain = t0 + TK <= sp.first;
-        const float tile_top = Q8 ? fmaxf(fmaxf(vs[TK], vs[TK + 1]), fmaxf(vs[TK + 2], vs[TK + 3])) : 0.f;
+        float tile_top = 0.f;
+        if (Q8)
+#pragma unroll
+          for (int k = 0; k < WIDENERS; ++k) tile_top = fmaxf(tile_top, vs[TK + k]);
         // tokens c .. c + 31 of the tile that this row sees: all in front of the drafted ones, then by the mask's bits
         auto seen = [&](int c) -> uint32_t {
           const int u0 = t0 + c - sp.first, k = u0 >> 5;          // drafted token of the first one
@@ -613,8 +617,9 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
     __syncwarp();
   } else if (warp >= 12) {
     // ================================ codes widened into tiles ===============================================
-    constexpr int CH = D / 16, RPI = 32 / CH, N = 32 / RPI;      // 16-byte pieces of a row; rows per access of the warp; accesses
-    const int c4 = warp - 12, r0 = lane / CH, c = lane % CH;      // this warp's 32 tokens of a tile start at 32 c4
+    constexpr int ROWS = TK / WIDENERS;                          // of a tile, per warp
+    constexpr int CH = D / 16, RPI = 32 / CH, N = ROWS / RPI;    // 16-byte pieces of a row; rows per access of the warp; accesses
+    const int c4 = warp - 12, r0 = lane / CH, c = lane % CH;      // this warp's tokens of a tile start at ROWS c4
     int seen = 0;
     bool ok = true;
     uint4 kr[N], vr[N];
@@ -624,7 +629,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
       const uint8_t* src = static_cast<const uint8_t*>(codes) + (int64_t)pc.b * sb + (int64_t)pc.h * sh + c * 16;
 #pragma unroll
       for (int i = 0; i < N; ++i) {
-        const int at = t0 + c4 * 32 + i * RPI + r0;
+        const int at = t0 + c4 * ROWS + i * RPI + r0;
         x[i] = make_uint4(0, 0, 0, 0);
         if (at < len) x[i] = __ldg(reinterpret_cast<const uint4*>(src + (int64_t)at * sl));
       }
@@ -632,7 +637,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
     auto store = [&](const uint4 (&x)[N], uint32_t dst) {
 #pragma unroll
       for (int i = 0; i < N; ++i) {
-        const int row = c4 * 32 + i * RPI + r0;
+        const int row = c4 * ROWS + i * RPI + r0;
         const uint32_t w[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
         uint32_t h[8];
 #pragma unroll
@@ -657,20 +662,20 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
       const float* ksg = p.k_scales + (int64_t)pc.b * p.ks_sb + (int64_t)pc.h * p.ks_sh;
       const float* vsg = p.v_scales + (int64_t)pc.b * p.vs_sb + (int64_t)pc.h * p.vs_sh;
       auto load_k = [&](int i) {
-        const int t0 = (pc.begin + i) * TK, at = t0 + c4 * 32 + lane;
+        const int t0 = (pc.begin + i) * TK, at = t0 + c4 * ROWS + lane;
         load(kr, p.k, p.k_sb, p.k_sh, p.k_sl, t0, sp.len);
-        ksr = at < sp.len ? __ldg(ksg + at) : 0.f;
+        ksr = lane < ROWS && at < sp.len ? __ldg(ksg + at) : 0.f;
       };
       auto load_v = [&](int i) {
-        const int t0 = (pc.begin + i) * TK, at = t0 + c4 * 32 + lane;
+        const int t0 = (pc.begin + i) * TK, at = t0 + c4 * ROWS + lane;
         load(vr, p.v, p.v_sb, p.v_sh, p.v_sl, t0, sp.len);
-        vsr = at < sp.len ? __ldg(vsg + at) : 0.f;
+        vsr = lane < ROWS && at < sp.len ? __ldg(vsg + at) : 0.f;
       };
       if (ntiles > 0) { load_k(0); load_v(0); }
       for (int i = 0; i < ntiles; ++i, ++seen) {
         const int stage = seen % STAGES;
         const uint32_t parity = ((uint32_t)(seen / STAGES) & 1u) ^ 1u;
-        float* ks = reinterpret_cast<float*>(sm + S::SCALES + stage * (2 * TK + 4) * 4);
+        float* ks = reinterpret_cast<float*>(sm + S::SCALES + stage * (2 * TK + WIDENERS) * 4);
         if (!(ok = wait(bar_kempty(stage), parity, 70))) break;
         store(kr, S::K + stage * S::TILE);
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -679,9 +684,9 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
         const float k_scale = ksr;
         if (i + 1 < ntiles) load_k(i + 1);
         if (!(ok = wait(bar_vempty(stage), parity, 71))) break;
-        const int at0 = (pc.begin + i) * TK + c4 * 32;
+        const int at0 = (pc.begin + i) * TK + c4 * ROWS;
         float v_scale = vsr;
-        if (CODE == XKV_CACHE_E4M3 && at0 + 32 > sp.first) {
+        if (CODE == XKV_CACHE_E4M3 && at0 + ROWS > sp.first) {
           // a NaN code among the drafted rows would reach rows that do not see it: the code becomes zero and the row's
           // scale the NaN, which the weights of hidden tokens leave out
           uint32_t bad = 0;
@@ -700,8 +705,10 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
           if (bad >> lane & 1u) v_scale = CUDART_NAN_F;
         }
         store(vr, S::V + stage * S::TILE);
-        ks[c4 * 32 + lane] = k_scale;
-        ks[TK + c4 * 32 + lane] = v_scale;
+        if (lane < ROWS) {
+          ks[c4 * ROWS + lane] = k_scale;
+          ks[TK + c4 * ROWS + lane] = v_scale;
+        }
         const uint32_t mag = __float_as_uint(v_scale) & 0x7fffffffu;
         const uint32_t top = __reduce_max_sync(0xffffffffu, mag < 0x7f800000u ? mag : 0u);
         if (lane == 0) ks[2 * TK + c4] = __uint_as_float(top);
