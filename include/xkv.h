@@ -71,6 +71,10 @@ typedef enum xkv_value_mode {
                                      kernel where the tcgen05 CTA-pair kernel would run (cross-checks) */
 #define XKV_FLAG_RECON_PAIR 16u  /* key reconstruction: ask for the CTA-pair variant where the
                                      library would not choose it by itself                    */
+#define XKV_FLAG_TREE_TCGEN05 64u /* xkv_tree_decode: ask for the tcgen05 kernel where the library would choose
+                                     another one that covers the call (cross-checks)          */
+#define XKV_FLAG_TREE_MMA_SYNC 128u /* xkv_tree_decode: keep the mma.sync kernel where the tcgen05 one would
+                                     run (cross-checks)                                       */
 
 /*
  * One decode-attention call.  Shapes (H = num_heads, KVH = num_kv_heads, L = kv_len):
@@ -349,7 +353,7 @@ XKV_API int xkv_cache_read(const xkv_cache_params* p, void* stream);
  *   q   (batch, num_heads, num_tokens, head_dim) of dtype
  *   k,v (batch, num_kv_heads, kv_len, head_dim): of dtype (XKV_CACHE_DENSE), or codes with k_scales / v_scales
  *   out (batch, num_heads * num_tokens, head_dim) of dtype: row h * num_tokens + t at o_sb, o_sr
- * Flags: XKV_FLAG_FORCE_GENERIC.  head_dim <= 256.  The status words at the start of the workspace are read with
+ * Flags: XKV_FLAG_FORCE_GENERIC, XKV_FLAG_TREE_TCGEN05, XKV_FLAG_TREE_MMA_SYNC.  head_dim <= 256.  The status words at the start of the workspace are read with
  * xkv_workspace_status, as for xkv_decode.
  */
 typedef struct xkv_tree_params {

@@ -286,7 +286,7 @@ def latent_append(latent, new_rows, proj, position):
 
 
 def _tree_decode(query, idx, KVH, L, k, ks, v, vs, scales, code, tree_mask, sm_scale, kv_lens, num_splits, force_generic,
-                 check_status):
+                 tcgen05, check_status):
     """Shared by the two tree entry points: k / v (bsz, KVH, L, head_dim) with strides ks / vs, `scales` the pointers and
     strides of the key and value scales."""
     b, H, T, D = query.shape
@@ -315,10 +315,13 @@ def _tree_decode(query, idx, KVH, L, k, ks, v, vs, scales, code, tree_mask, sm_s
     if qs[3] != 1 and D != 1:
         q = query.contiguous()
         qs = q.stride()
+    flags = _C.FLAG_FORCE_GENERIC if force_generic else 0
+    if tcgen05 is not None:      # None: the library chooses; True / False pin the tcgen05 or the mma.sync kernel
+        flags |= _C.FLAG_TREE_TCGEN05 if tcgen05 else _C.FLAG_TREE_MMA_SYNC
     device = q.device
     out = torch.empty_like(q) if q.is_contiguous() else torch.empty((b, H, T, D), dtype=q.dtype, device=device)
     _C.run_tree_decode(_C.TREE_PARAMS.pack(
-        dtype, code, _C.FLAG_FORCE_GENERIC if force_generic else 0, b, H, KVH, T, L, D, num_splits,
+        dtype, code, flags, b, H, KVH, T, L, D, num_splits,
         D ** -0.5 if sm_scale is None else sm_scale, len_ptr, tm_ptr, tm_sb, tm_st, q.data_ptr(), qs[0], qs[1], qs[2],
         k.data_ptr(), ks[0], ks[1], ks[2], v.data_ptr(), vs[0], vs[1], vs[2], *scales, out.data_ptr(), H * T * D, D),
         device, idx, check_status)
@@ -326,7 +329,7 @@ def _tree_decode(query, idx, KVH, L, k, ks, v, vs, scales, code, tree_mask, sm_s
 
 
 def group_query_attention_tree(query, key, value, tree_mask=None, *, sm_scale=None, kv_lens=None, num_splits=0,
-                               force_generic=False, check_status=None):
+                               force_generic=False, tcgen05=None, check_status=None):
     """Attention of a tree of drafted tokens over a dense cache (the verification step of speculative decoding).
 
     query (bsz, num_heads, T, head_dim); key / value (bsz, num_kv_heads, kv_len, head_dim), head_dim <= 256, any strides
@@ -352,11 +355,11 @@ def group_query_attention_tree(query, key, value, tree_mask=None, *, sm_scale=No
         value = value.contiguous()
         vs = value.stride()
     return _tree_decode(query, idx, shape[1], shape[2], key, ks, value, vs, (0, 0, 0, 0, 0, 0), _C.CACHE_DENSE, tree_mask,
-                        sm_scale, kv_lens, num_splits, force_generic, check_status)
+                        sm_scale, kv_lens, num_splits, force_generic, tcgen05, check_status)
 
 
 def group_query_attention_quantized(query, cache, tree_mask=None, *, sm_scale=None, kv_lens=None, num_splits=0,
-                                    force_generic=False, check_status=None):
+                                    force_generic=False, tcgen05=None, check_status=None):
     """Decode attention over an 8-bit cache (a QuantizedCache), read as it is held: the codes are widened in registers
     and the scales applied to logits and probabilities.  query (bsz, num_heads, T, head_dim), T = 1 for a plain decode
     step, float32, bfloat16 or float16.  kv_lens, tree_mask and sm_scale as in group_query_attention_tree (kv_lens
@@ -368,7 +371,7 @@ def group_query_attention_quantized(query, cache, tree_mask=None, *, sm_scale=No
         raise ValueError(f"query must be ({b}, num_heads, T, {D}); got {tuple(shape)}")
     scales = (cache.key_scales.data_ptr(), kss[0], kss[1], cache.value_scales.data_ptr(), vss[0], vss[1])
     return _tree_decode(query, idx, KVH, cap, cache.key_codes, ks, cache.value_codes, vs, scales, code, tree_mask, sm_scale,
-                        kv_lens, num_splits, force_generic, check_status)
+                        kv_lens, num_splits, force_generic, tcgen05, check_status)
 
 
 def xkv_group_decode(queries, key_A, key_Bs, value, value_Bs=None, *, theta, sm_scale=None,

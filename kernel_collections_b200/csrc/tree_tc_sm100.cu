@@ -776,6 +776,12 @@ bool map_ok(const void* ptr, int64_t stride, int n, bool zero = true) {
 bool tree_tc_supported(const xkv_tree_params& p, int rows) {
   using namespace tree;
   if (p.dtype == XKV_F32 || rows <= 16 || p.num_tokens > MAX_T) return false;
+  // The stream kernel reads the cache once per 16 rows, this one once, but it takes some 8 us longer to set up (tensor
+  // memory, operands in shared memory, three meetings per strip): SETUP bytes of reading.  R = 24 over 8 heads of 1023
+  // 16-bit rows (4 MB): 17 us there, 25 here; R = 104 over 8 x 16384 rows (537 MB): 405 us there, 125 here.
+  constexpr double SETUP = 48e6;
+  const double bytes = 2.0 * p.batch * p.num_kv_heads * p.kv_len * p.head_dim * (p.cache_code == XKV_CACHE_DENSE ? 2 : 1);
+  if ((p.flags & XKV_FLAG_TREE_MMA_SYNC) || (!(p.flags & XKV_FLAG_TREE_TCGEN05) && bytes * (ceil_div(rows, 16) - 1) < SETUP)) return false;
   if (p.cache_code != XKV_CACHE_DENSE) return true;      // beyond what tree_stream_supported() has checked
   return map_ok(p.k, p.k_sb, p.batch) && map_ok(p.k, p.k_sh, p.num_kv_heads) && map_ok(p.k, p.k_sl, 2, false) &&
          map_ok(p.v, p.v_sb, p.batch) && map_ok(p.v, p.v_sh, p.num_kv_heads) && map_ok(p.v, p.v_sl, 2, false);

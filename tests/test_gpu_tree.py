@@ -17,6 +17,16 @@ from kernel_collections_b200 import _C
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
+PIN = None
+
+
+@pytest.fixture(autouse=True, params=[None, True], ids=["chosen", "tcgen05"])
+def pinned(request):
+    """Every test on the kernel that the library chooses, and on the tcgen05 kernel where it covers the call (the
+    library keeps it for larger caches than most tests have)."""
+    global PIN
+    PIN = request.param
+    yield
 
 
 def random_tree(g, n):
@@ -91,6 +101,7 @@ def case(seed, b, H, KVH, T, L, D, dtype, code, mask_kind="tree", lens=None):
 
 def run(q, k, v, mask, lens, code, scale=None, **kw):
     """Through the public entry points; returns the output and the float64 key / value rows that the cache holds."""
+    kw.setdefault("tcgen05", PIN)
     lt = None if lens is None else torch.tensor(lens, dtype=torch.int32, device=DEV)
     m = None if mask is None else mask.to(DEV)
     if code == "dense":
@@ -264,13 +275,14 @@ def test_strided_and_unaligned_caches_and_queries(dtype, T):
     odd = lambda t: torch.cat([t[..., :1], t], -1).to(DEV)[..., 1:]  # noqa: E731
     flip = lambda t: t.transpose(2, 3).contiguous().to(DEV).transpose(2, 3)  # noqa: E731
     for f in (tok, wide, flip):
-        assert torch.equal(K.group_query_attention_tree(f(q), f(k), f(v), m), want)
+        assert torch.equal(K.group_query_attention_tree(f(q), f(k), f(v), m, tcgen05=PIN), want)
     out = K.group_query_attention_tree(odd(q), odd(k), odd(v), m)      # another kernel: compare with 64 bits
     close(out, q, k.double(), v.double(), mask, [L] * b, D ** -0.5, False)
     m2 = torch.zeros(b, T, 2 * T, dtype=torch.bool, device=DEV)
     m2[:, :, ::2] = m
-    assert torch.equal(K.group_query_attention_tree(q.to(DEV), k.to(DEV), v.to(DEV), m2[:, :, ::2]), want)
-    shared = K.group_query_attention_tree(q.to(DEV), k[:1].to(DEV).expand(b, -1, -1, -1), v[:1].to(DEV).expand(b, -1, -1, -1), m)
+    assert torch.equal(K.group_query_attention_tree(q.to(DEV), k.to(DEV), v.to(DEV), m2[:, :, ::2], tcgen05=PIN), want)
+    shared = K.group_query_attention_tree(q.to(DEV), k[:1].to(DEV).expand(b, -1, -1, -1), v[:1].to(DEV).expand(b, -1, -1, -1), m,
+                                          tcgen05=PIN)
     assert torch.equal(shared[0], want[0])
 
 
@@ -281,11 +293,11 @@ def test_strided_quantised_cache(code, T):
     q, k, v, mask, _ = case(8, b, H, KVH, T, L, D, torch.bfloat16, code, "trees")
     c = K.quantized_cache(b, KVH, L, D, code=code)
     K.quantized_cache_append(c, k.to(DEV), v.to(DEV), 0)
-    want = K.group_query_attention_quantized(q.to(DEV), c, mask.to(DEV))
+    want = K.group_query_attention_quantized(q.to(DEV), c, mask.to(DEV), tcgen05=PIN)
     tok = lambda t: t.view(torch.uint8).transpose(1, 2).contiguous().transpose(1, 2).view(t.dtype)  # noqa: E731
     pad = lambda t: torch.cat([t, t[..., :5]], -1)[..., :L]  # noqa: E731
     c2 = K.QuantizedCache(tok(c.key_codes), pad(c.key_scales), tok(c.value_codes), pad(c.value_scales))
-    assert torch.equal(K.group_query_attention_quantized(q.to(DEV), c2, mask.to(DEV)), want)
+    assert torch.equal(K.group_query_attention_quantized(q.to(DEV), c2, mask.to(DEV), tcgen05=PIN), want)
 
 
 @pytest.mark.parametrize("code", CODES)
@@ -296,7 +308,7 @@ def test_split_counts_repeats_and_the_portable_kernel_agree(code, T):
     first, kd, vd = run(q, k, v, mask, None, code)
     again, _, _ = run(q, k, v, mask, None, code)
     assert torch.equal(first, again)
-    for kw in (dict(num_splits=1), dict(num_splits=3), dict(num_splits=64), dict(force_generic=True)):
+    for kw in (dict(num_splits=1), dict(num_splits=3), dict(num_splits=64), dict(force_generic=True), dict(tcgen05=False)):
         out, _, _ = run(q, k, v, mask, None, code, **kw)
         close(out, q, kd, vd, mask, [L], D ** -0.5, code != "dense")
 
@@ -311,11 +323,11 @@ def test_captured_calls_replay_and_two_graphs_run_side_by_side(code, G, T):
         want, _, _ = run(q, k, v, mask, None, code)
         qd, kd, vd, md = q.to(DEV), k.to(DEV), v.to(DEV), mask.to(DEV)
         if code == "dense":
-            call = lambda qd=qd, kd=kd, vd=vd, md=md: K.group_query_attention_tree(qd, kd, vd, md)  # noqa: E731
+            call = lambda qd=qd, kd=kd, vd=vd, md=md: K.group_query_attention_tree(qd, kd, vd, md, tcgen05=PIN)  # noqa: E731
         else:
             c = K.quantized_cache(b, KVH, L, D, code=code)
             K.quantized_cache_append(c, kd, vd, 0)
-            call = lambda qd=qd, c=c, md=md: K.group_query_attention_quantized(qd, c, md)  # noqa: E731
+            call = lambda qd=qd, c=c, md=md: K.group_query_attention_quantized(qd, c, md, tcgen05=PIN)  # noqa: E731
         graph = torch.cuda.CUDAGraph()
         with torch.cuda.graph(graph):
             out = call()
@@ -343,7 +355,7 @@ def test_another_stream_and_no_sync_between_calls():
         s = torch.cuda.Stream()
         with torch.cuda.stream(s):
             for _ in range(4):
-                outs.append(K.group_query_attention_tree(qd, kd, vd, md))
+                outs.append(K.group_query_attention_tree(qd, kd, vd, md, tcgen05=PIN))
     torch.cuda.synchronize()
     assert all(torch.equal(o, want) for o in outs)
 
@@ -358,7 +370,7 @@ def test_a_long_cache_past_32_bit_offsets():
     tail = torch.randn(2, KVH, n, D, generator=g, device=DEV).half()
     k[:, :, L - n:] = tail
     q = (torch.randn(2, 16, 2, D, generator=g, device=DEV) * 4).half()
-    out = K.group_query_attention_tree(q, k, k, sm_scale=1.0)
+    out = K.group_query_attention_tree(q, k, k, sm_scale=1.0, tcgen05=PIN)
     s = torch.einsum("bhgtd,bhld->bhgtl", q.double().view(2, KVH, 2, 2, D), tail.double())
     s[:, :, :, 0, n - 1] = -float("inf")
     zeros = float(L - n)
@@ -409,7 +421,7 @@ def test_a_verification_step_rotates_writes_and_attends():
         depth = mask.sum(-1).to(torch.int32) - 1
         qr = step(T, lens[:, None] + depth, lens, None)
         lens = lens + T
-        out = K.group_query_attention_quantized(qr, cache, mask.to(DEV), kv_lens=lens.to(DEV))
+        out = K.group_query_attention_quantized(qr, cache, mask.to(DEV), kv_lens=lens.to(DEV), tcgen05=PIN)
         kd, vd = dense_of(cache.key_codes, cache.key_scales), dense_of(cache.value_codes, cache.value_scales)
         close(out, qr, kd, vd, mask, lens.tolist(), D ** -0.5, True)
     # what was written reads back as what the attention saw

@@ -113,3 +113,19 @@ def test_cpu_tensors_are_rejected():
         K.quantized_cache_append(c, k, k, 0)
     with pytest.raises(RuntimeError, match="CUDA"):
         K.rotary_embedding(q, k[:, :, :2], K.rotary_frequencies(64, device="cpu")[0], 0)
+
+
+def test_kernel_selection_follows_the_call():
+    lib = _C.load()
+    plan = lambda **kw: lib.xkv_tree_decode_plan(tree(**kw))  # noqa: E731
+    q8 = dict(code=1, ks=A, vs=A)
+    assert plan(tokens=1) == b"stream" and plan(tokens=1, **q8) == b"stream"
+    assert plan(head_dim=96) == b"portable" and plan(dtype=0) == b"portable" and plan(k=A + 2) == b"portable"
+    assert plan(dtype=0, **q8) == b"stream" and plan(dtype=0, tokens=64, kv_len=100000, **q8) == b"stream"
+    assert plan(flags=_C.FLAG_FORCE_GENERIC) == b"portable"
+    # more than 16 query rows per KV head: tcgen05 once re-reading the cache costs more than its set-up
+    assert plan(tokens=8, kv_len=1000) == b"stream" and plan(tokens=8, kv_len=100000) == b"tree_tc"
+    assert plan(tokens=8, kv_len=1000, flags=_C.FLAG_TREE_TCGEN05) == b"tree_tc"
+    assert plan(tokens=8, kv_len=100000, flags=_C.FLAG_TREE_MMA_SYNC) == b"stream"
+    assert plan(tokens=4, kv_len=100000, flags=_C.FLAG_TREE_TCGEN05) == b"stream"       # 16 rows
+    assert plan(tokens=257, kv_len=100000) == b"stream"
