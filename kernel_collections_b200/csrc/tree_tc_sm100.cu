@@ -47,7 +47,8 @@ struct Smem {
   static constexpr int MASK = SCALES + STAGES * (2 * TK + WIDENERS) * 4;   // [token][words]
   static constexpr int BAD = MASK + MAX_T * (MAX_T / 32) * 4;   // drafted tokens with values that are not finite
   static constexpr int ML = BAD + MAX_T / 32 * 4;               // [128] of the second group, MB == 1
-  static constexpr int BAR = ML + TK * 8;
+  static constexpr int SCALE = ML + TK * 8;                     // [row] of the strip: factor on its scores
+  static constexpr int BAR = SCALE + 2 * TK * 4;
   static constexpr int MISC = BAR + 16 * 8;
   static constexpr int BYTES = MISC + 16 + 1024;
 };
@@ -170,6 +171,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
     uint32_t* mask_s = reinterpret_cast<uint32_t*>(sm + S::MASK);
     uint32_t* bad_s = reinterpret_cast<uint32_t*>(sm + S::BAD);
     float2* ml_s = reinterpret_cast<float2*>(sm + S::ML);
+    float* scale_s = reinterpret_cast<float*>(sm + S::SCALE);
     float* join_s = reinterpret_cast<float*>(sm + S::Q);    // [dim][row] of the second group, MB == 1
     uint32_t q_phase = 0, end_phase = 0, s_phase = 0;
     int tiles_seen = 0;                                     // of the pieces before
@@ -200,34 +202,42 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
       const bool busy = (pc.rb * MB + blk) * 128 + (warp & 3) * 32 < a.rows;      // some row of this warp is one
       float row_scale = 1.f;
       {
-        // a warp takes its 32 rows one after the other, so that the reads are contiguous; lane i keeps row i's scale
+        // a warp takes its rows one after the other, so that the reads are contiguous; MB == 1: the groups hold the same
+        // rows and take half of them each
         constexpr int PER = D / 32, AHEAD = 16;
         const bool wide = reinterpret_cast<uintptr_t>(p.q) % (PER * 2) == 0 && p.q_sb % PER == 0 && p.q_sh % PER == 0 && p.q_st % PER == 0;
-        struct alignas(PER * 2) Few { T x[PER]; };
-        const int first_row = (pc.rb * MB + blk) * 128 + (warp & 3) * 32;
-        int qh = first_row / T_, qt = first_row - qh * T_;
+        using Few = typename std::conditional<PER == 4, uint2, uint32_t>::type;       // a lane's PER elements
+        const int first_row = (pc.rb * MB + blk) * 128 + (warp & 3) * 32, from_row = first_row + (MB == 1 ? w * 16 : 0);
+        int qh = from_row / T_, qt = from_row - qh * T_;
+        const int64_t next_head = p.q_sh - (T_ - 1) * p.q_st;   // from a head's last token to the next head's first
         const T* src = static_cast<const T*>(p.q) + (int64_t)pc.b * p.q_sb + (int64_t)(pc.h * G + qh) * p.q_sh + (int64_t)qt * p.q_st + lane * PER;
-        for (int i0 = 0; i0 < 32 && busy; i0 += AHEAD) {
-          Few q[AHEAD];
+        for (int i0 = MB == 1 ? w * 16 : 0; i0 < (MB == 1 ? w * 16 + 16 : 32) && busy; i0 += AHEAD) {
+          Few q[AHEAD] = {};
+          auto rows = [&](auto read) {
 #pragma unroll
-          for (int i = 0; i < AHEAD; ++i) {
-            const int qr = first_row + i0 + i;
-#pragma unroll
-            for (int e = 0; e < PER; ++e) q[i].x[e] = from_float<T>(0.f);
-            if (qr < a.rows) {
-              if (wide) q[i] = *reinterpret_cast<const Few*>(src);
-              else
-#pragma unroll
-                for (int e = 0; e < PER; ++e) q[i].x[e] = src[e];
-              src += p.q_st;
-              if (++qt == T_) {
-                qt = 0;
-                src += p.q_sh - T_ * p.q_st;
-              }
+            for (int i = 0; i < AHEAD; ++i) {
+              if (first_row + i0 + i < a.rows) q[i] = read(src);
+              const bool last = ++qt == T_;
+              qt = last ? 0 : qt;
+              src += last ? next_head : p.q_st;
             }
+          };
+          if (wide) {
+            rows([](const T* s) { return *reinterpret_cast<const Few*>(s); });
+          } else {
+            rows([](const T* s) {
+              Few f;
+              T* x = reinterpret_cast<T*>(&f);
+#pragma unroll
+              for (int e = 0; e < PER; ++e) x[e] = s[e];
+              return f;
+            });
           }
 #pragma unroll
           for (int i = 0; i < AHEAD; ++i) {
+            float2 x[PER / 2];
+#pragma unroll
+            for (int e = 0; e < PER / 2; ++e) x[e] = TypeTraits<T>::unpack2(reinterpret_cast<const uint32_t*>(&q[i])[e]);
             // the sign of the scale goes to the queries, so that the largest product is the largest score; a scale of zero too
             float up = a.scale_log2 < 0.f ? -1.f : 1.f, scale = fmaxf(fabsf(a.scale_log2), 1.17549435e-38f);
             if (a.scale_log2 == 0.f) {
@@ -236,7 +246,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
             } else if (Q8) {
               float top = 0.f;
 #pragma unroll
-              for (int e = 0; e < PER; ++e) top = fmaxf(top, fabsf(to_float(q[i].x[e])));
+              for (int e = 0; e < PER / 2; ++e) top = fmaxf(top, fmaxf(fabsf(x[e].x), fabsf(x[e].y)));
               top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top)));
               if (top > 0.f && top < CUDART_INF_F) {
                 const int e = min(max(14 - (int)(((__float_as_uint(top) >> 23) & 255u)) + 127, -120), 120);
@@ -244,12 +254,12 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
                 scale = fmaxf(scale * __uint_as_float((uint32_t)(127 - e) << 23), 1.17549435e-38f);
               }
             }
-            if (lane == i0 + i) row_scale = scale;
             const int rr = (warp & 3) * 32 + i0 + i, d = lane * PER;
             uint32_t* to = reinterpret_cast<uint32_t*>(sm + S::Q + blk * S::TILE + (d >> 6) * BOX + rr * 128 +
                                                        ((((d & 63) >> 3) ^ (rr & 7)) << 4) + (d & 7) * 2);
 #pragma unroll
-            for (int e = 0; e < PER; e += 2) to[e / 2] = TypeTraits<M>::pack2(to_float(q[i].x[e]) * up, to_float(q[i].x[e + 1]) * up);
+            for (int e = 0; e < PER / 2; ++e) to[e] = TypeTraits<M>::pack2(x[e].x * up, x[e].y * up);
+            if (lane == 0) scale_s[blk * 128 + rr] = scale;
           }
         }
         if ((pc.begin + ntiles) * TK > sp.first) {            // drafted tokens in this piece
@@ -266,6 +276,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
         arrive(bar_q);
         if (!(ok = wait(bar_q, q_phase, 50))) break;
         q_phase ^= 1u;
+        if (busy) row_scale = scale_s[blk * 128 + r];
       }
       float ref = -CUDART_INF_F, unit = 0.f;
       float2 l = make_float2(0.f, 0.f);
