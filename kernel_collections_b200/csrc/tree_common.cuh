@@ -8,9 +8,9 @@
 // Work is dealt in units of `unit_tokens` cache rows.  All units of all strips form one line, cut into equal shares for
 // the blocks of a single wave: sequences of any lengths keep every block equally busy, and one long sequence is spread
 // over all of them.  The lengths are on the device, so every block finds its own share (a scan over the batch).  A
-// block's stretch of one strip is a piece; block c's piece of strip s has the number c + s, which is unique because along
-// the line c and s never decrease and one of them grows from piece to piece.  A piece that covers its strip is finished by
-// its block.  Otherwise it leaves, per row, its unnormalised output and (m, l): the reference of the exponents in the log2
+// block's stretch of one strip is a piece.  A piece that covers its strip is finished by its block.  At most two pieces of a
+// block do not: its first, which goes on with a strip that another block began, and its last, which begins one; block c
+// keeps them in the places 2c and 2c + 1.  Of such a piece it leaves, per row, the unnormalised output and (m, l): the reference of the exponents in the log2
 // domain and the sum of exp2(score - m), and the merge joins a strip's pieces in their order.
 #pragma once
 #include "xkv_internal.h"
@@ -27,8 +27,8 @@ struct Args {
   int unit_tokens;
   int grid;                // blocks that share the units
   float scale_log2;        // sm_scale * log2(e)
-  float* part_o;           // [piece][block_rows][head_dim]
-  float2* part_ml;         // [piece][block_rows]
+  float* part_o;           // [place][block_rows][head_dim]
+  float2* part_ml;         // [place][block_rows]
   int* status;
   int map_b[2], map_h[2];  // tensor maps of K and V: 0 where the sequences / KV heads share one (stride 0)
 };
@@ -132,7 +132,7 @@ struct Piece {
   int b, h, rb;              // sequence, KV head, row block
   int begin, end;            // units
   bool whole;                // covers its strip
-  int64_t id;
+  int64_t id;                // its place among the partial results
 };
 struct Walk {
   int64_t x, stop;
@@ -161,7 +161,7 @@ __device__ __forceinline__ bool next_piece(const Args& a, Walk& w, Piece& pc) {
   pc.begin = (int)(y - (int64_t)strip * w.at.units);
   pc.end = (int)min((int64_t)w.at.units, pc.begin + (w.stop - w.x));
   pc.whole = pc.begin == 0 && pc.end == w.at.units;
-  pc.id = (int64_t)blockIdx.x + (int64_t)w.at.b * per + strip;
+  pc.id = 2 * (int64_t)blockIdx.x + (pc.begin == 0);
   w.x += pc.end - pc.begin;
   return true;
 }

@@ -225,13 +225,11 @@ __global__ void __launch_bounds__(128) merge_kernel(const Args a) {
   const int first = (int)(begin / line.share), last = (int)((begin + at.units - 1) / line.share);
   asm volatile("griddepcontrol.wait;" ::: "memory");      // the pieces
   if (first == last) return;                              // one piece: its block has written the row
-  const int64_t id = first + (int64_t)b * p.num_kv_heads * a.blocks + strip;
   const int n = last - first + 1, rr = r % a.block_rows;
-  const float2* ml = a.part_ml + id * a.block_rows + rr;
-  const float* po = a.part_o + (id * a.block_rows + rr) * D;
-  const int64_t ml_step = a.block_rows, po_step = (int64_t)a.block_rows * D;
+  // row of piece i among the partial results: the strip begins in block `first` (its second place)
+  auto place = [&](int i) { return (2 * (int64_t)(first + i) + (i == 0)) * a.block_rows + rr; };
   float M = -CUDART_INF_F;
-  for (int i = lane; i < n; i += 32) M = fmaxf(M, ml[i * ml_step].x);
+  for (int i = lane; i < n; i += 32) M = fmaxf(M, a.part_ml[place(i)].x);
 #pragma unroll
   for (int o = 16; o; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
   if (M == -CUDART_INF_F) M = 0.f;
@@ -250,9 +248,10 @@ __global__ void __launch_bounds__(128) merge_kernel(const Args a) {
         x[k] = make_float2(-CUDART_INF_F, 0.f);
         y[k] = make_float4(0.f, 0.f, 0.f, 0.f);
         if (i < n) {
-          x[k] = ml[i * ml_step];
-          if (d < D && quads) y[k] = *reinterpret_cast<const float4*>(po + i * po_step + d);
-          else if (d < D) y[k].x = po[i * po_step + d];
+          const int64_t at = place(i);
+          x[k] = a.part_ml[at];
+          if (d < D && quads) y[k] = *reinterpret_cast<const float4*>(a.part_o + at * D + d);
+          else if (d < D) y[k].x = a.part_o[at * D + d];
         }
       }
 #pragma unroll
@@ -351,7 +350,7 @@ bool make_plan(const xkv_tree_params& p, TreePlan* pl) {
   pl->grid = (int)grid;
   pl->merged = units > 1;
   size_t off = 256;
-  const size_t rows = pl->merged ? (size_t)(grid + strips) * pl->block_rows : 0;
+  const size_t rows = pl->merged ? (size_t)(2 * grid) * pl->block_rows : 0;
   pl->off_o = off;
   off += align_up(rows * p.head_dim * sizeof(float), 256);
   pl->off_ml = off;

@@ -23,6 +23,9 @@
 //    (it cancels in O / l) so that those down to 2^-20 of the largest keep all 11 bits, and the value scales are taken
 //    relative to a power of two above the largest seen.
 //  * fp32 queries: Q and P in two fp16 terms each (22 bits), two MMAs instead of one.
+// 4 x 131071 rows of 8 heads (e4m3, 8 query rows per head, 1.1 GB): 173 us, 6.4 TB/s; the same in int8, with 16 query rows or
+// with fp32 queries within 5 %.  16 ragged sequences of up to 16384 int8 rows (0.42 GB): 78 us.  One sequence of 777 rows: 18 us,
+// the host's time for the call's two launches.
 #include "tree_common.cuh"
 #include "sm100_common.cuh"
 #include <type_traits>
@@ -131,7 +134,7 @@ __global__ void __launch_bounds__(NT, 1) stream_kernel(const Args a) {
   constexpr int E = WIDE ? 2 : 1;                  // tokens of every 8 that a thread scores, for each of its rows
   constexpr int QV = WIDE ? 1 : 2;                 // k-steps per 16 bytes of query operand
   // weights are 2^(score - reference + LIFT); the reference follows the maximum when it is passed by more than SLACK
-  constexpr float LIFT = std::is_same<M, __half>::value ? 6.f : 0.f, SLACK = std::is_same<M, __half>::value ? 9.f : 32.f;
+  constexpr float LIFT = std::is_same<M, __half>::value ? 6.f : -12.f, SLACK = std::is_same<M, __half>::value ? 9.f : 20.f;
   extern __shared__ __align__(128) uint8_t smem[];
   const xkv_tree_params& p = a.p;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;

@@ -16,6 +16,11 @@
 // taken against the old reference while the new maximum is formed, kept in registers, and taken again in the rare tile that
 // moves a reference or holds drafted tokens.  Number ranges (query scaling, LIFT, value scales relative to a power of two) are those of
 // tree_stream_sm100.cu.  P is rounded to the 16-bit type of the product and l sums the rounded values.
+// What bounds it.  Per 128 x 128 item the tensor core needs 1024 cycles and the exponentials 1024 of the 16-per-clock unit; a
+// group's chain (softmax 1800, then P.V and S with their latencies 1400) leaves about 2000 per item.  512 fp16 rows over
+// 4 x 32768 rows of 8 heads: 16-bit cache 323 us (852 TFLOP/s), int8 461 us (596: widening, scales and softmax share the issue
+// slots).  104 rows over 8 x 16384 ragged bf16 rows: 100 us, steady tiles at the rate of HBM, the rest set-up and ends of the
+// strips.  Handing the exponentials from one group to the other in strict turns was measured slower (536 us against 474).
 // All waits are bounded; a group that gives up raises the abort flag, which ends the others' waits.
 #include "tree_common.cuh"
 #include "sm100_common.cuh"
@@ -107,8 +112,9 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
   using M = typename std::conditional<Q8, __half, T>::type;
   using S = Smem<D, MB>;
   // weights are 2^(score - reference + LIFT); the reference follows the maximum when it is passed by more than SLACK
-  // (fp16: below 2^15 always, and all 11 bits down to 2^-20 of the reference; bf16 has the range of fp32)
-  constexpr float LIFT = std::is_same<M, __half>::value ? 6.f : 0.f, SLACK = std::is_same<M, __half>::value ? 9.f : 32.f;
+  // (fp16: below 2^15 always, and all 11 bits down to 2^-20 of the reference; bf16 has the range of fp32, and stays below 2^8
+  // so that products with large values do)
+  constexpr float LIFT = std::is_same<M, __half>::value ? 6.f : -12.f, SLACK = std::is_same<M, __half>::value ? 9.f : 20.f;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw = smem_u32(smem_raw);
   const uint32_t base = (raw + 1023u) & ~1023u;

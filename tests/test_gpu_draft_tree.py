@@ -136,7 +136,7 @@ def test_one_token_and_a_tree_at_every_head_size(dtype, code, D):
 @pytest.mark.parametrize("code", CODES)
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("G,T", [(1, 1), (1, 16), (5, 3), (4, 4), (1, 17), (8, 4), (4, 16), (3, 21), (8, 16), (1, 129),
-                                 (5, 26), (8, 64)])
+                                 (5, 26), (8, 64), (1, 300)])
 def test_row_counts(dtype, code, G, T):
     """G heads per KV head times T drafted tokens: below, at and above the row blocks of every kernel."""
     check(G * 100 + T, 2, 2 * G, 2, T, 413, 128, dtype, code, "trees")
