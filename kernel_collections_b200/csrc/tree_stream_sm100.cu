@@ -24,8 +24,8 @@
 //    relative to a power of two above the largest seen.
 //  * fp32 queries: Q and P in two fp16 terms each (22 bits), two MMAs instead of one.
 // 4 x 131071 rows of 8 heads (e4m3, 8 query rows per head, 1.1 GB): 173 us, 6.4 TB/s; the same in int8, with 16 query rows or
-// with fp32 queries within 5 %.  16 ragged sequences of up to 16384 int8 rows (0.42 GB): 78 us.  One sequence of 777 rows: 18 us,
-// the host's time for the call's two launches.
+// with fp32 queries within 5 %.  16 ragged sequences of up to 16384 int8 rows (0.42 GB): 78 us.  One sequence of 777 rows: 15 us,
+// the host's time for the call.
 #include "tree_common.cuh"
 #include "sm100_common.cuh"
 #include <type_traits>
@@ -145,7 +145,8 @@ __global__ void __launch_bounds__(NT, 1) stream_kernel(const Args a) {
   while (next_piece(a, walk, pc)) {
     const int b = pc.b, h = pc.h, rb = pc.rb;
     const Span sp = span_of(p, b);
-    const int begin = pc.begin, end = pc.end;
+    const int mult = a.unit_tokens / S::UNIT;        // tiles of all warps per unit of the line
+    const int begin = pc.begin * mult, end = min(pc.end * mult, (sp.len + S::UNIT - 1) / S::UNIT);
 
     uint8_t* const ring = smem + warp * (STAGES * S::STAGE);
     const uint32_t ring_a = smem_u32(ring);
@@ -690,6 +691,13 @@ void tree_stream_plan(const xkv_tree_params& p, TreePlan* pl) {
   pl->block_rows = pl->rows <= 8 ? 8 : 16;
   pl->unit_tokens = tree::NW * tree::HALF / (p.head_dim * (p.cache_code == XKV_CACHE_DENSE ? 2 : 1));
   pl->slots = device_sm_count();
+  // A short cache is one unit, so that no strip is cut and nothing has to be merged: up to LAUNCH tiles in a row cost a
+  // block about what the merge and its launch cost the call (777 int8 rows, 4 tiles: 18.4 -> 15.2 us per queued call; 1023
+  // bf16 rows, 8 tiles: 17.0 -> 14.4; a call that is waited for, 30 -> 33).
+  constexpr int LAUNCH = 8;
+  const int tiles = ceil_div(p.kv_len, pl->unit_tokens);
+  const int64_t strips = (int64_t)p.batch * p.num_kv_heads * ceil_div(pl->rows, pl->block_rows);
+  if (tiles <= LAUNCH && strips <= pl->slots && p.num_splits == 0) pl->unit_tokens *= tiles;
 }
 
 int tree_stream_decode(const tree::Args& a, cudaStream_t st) {
