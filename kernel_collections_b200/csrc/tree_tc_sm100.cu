@@ -18,7 +18,7 @@
 // tree_stream_sm100.cu.  P is rounded to the 16-bit type of the product and l sums the rounded values.
 // What bounds it.  Per 128 x 128 item the tensor core needs 1024 cycles and the exponentials 1024 of the 16-per-clock unit; a
 // group's chain (softmax 1800, then P.V and S with their latencies 1400) leaves about 2000 per item.  512 fp16 rows over
-// 4 x 32768 rows of 8 heads: 16-bit cache 323 us (852 TFLOP/s), int8 461 us (596: the softmax waits for scales from shared memory).  104 rows over 8 x 16384 ragged bf16 rows: 100 us, steady tiles at the rate of HBM, the rest set-up and ends of the
+// 4 x 32768 rows of 8 heads: 16-bit cache 323 us (852 TFLOP/s), int8 450 us (611: the softmax waits for scales from shared memory).  104 rows over 8 x 16384 ragged bf16 rows: 100 us, steady tiles at the rate of HBM, the rest set-up and ends of the
 // strips.  Handing the exponentials from one group to the other in strict turns was measured slower (536 us against 474).
 // All waits are bounded; a group that gives up raises the abort flag, which ends the others' waits.
 #include "tree_common.cuh"
@@ -83,6 +83,11 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
 }
 template <typename T> __device__ __forceinline__ float to_float(T v) { return TypeTraits<T>::to_f(v); }
 template <typename T> __device__ __forceinline__ T from_float(float v) { return TypeTraits<T>::from_f(v); }
+
+// The value scales are taken relative to a power of two above the largest seen, at least this one (weights divided by it, and
+// their sums, stay below 2^127).  The division is part of the exponent, and O and l carry it alike.
+constexpr float SMALLEST_UNIT = 8.0779357e-28f;      // 2^-90
+__device__ __forceinline__ float log2_of(float power_of_two) { return (float)((int)(__float_as_uint(power_of_two) >> 23) - 127); }
 
 // one lane of the warp, the same one every time
 __device__ __forceinline__ bool elect() {
@@ -283,7 +288,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
         q_phase ^= 1u;
         if (busy) row_scale = scale_s[blk * 128 + r];
       }
-      float ref = -CUDART_INF_F, unit = 0.f;
+      float ref = -CUDART_INF_F, unit = SMALLEST_UNIT;       // unit: the power of two that the value scales are relative to
       float2 l = make_float2(0.f, 0.f);
       int items = 0;
       for (int i = MB == 2 ? 0 : w; i < ntiles; i += MB == 2 ? 1 : 2, ++items) {
@@ -325,14 +330,12 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
               }
             }
           };
-          float b1, inv = 1.f;
-          auto settle = [&]() {                               // what follows from ref and unit
-            b1 = ref == -CUDART_INF_F ? 0.f : LIFT - ref;
-            if (Q8) inv = unit > 0.f ? 1.f / unit : 0.f;
-          };
+          float b1;                                           // weights are 2^(score + b1), over 8-bit caches divided by unit
+          auto settle = [&]() { b1 = ref == -CUDART_INF_F ? 0.f : LIFT - ref - (Q8 ? log2_of(unit) : 0.f); };
           settle();
           // their weights against the reference, packed, and the sum of them
           auto weights = [&](int c, const float2 (&x)[16], uint32_t bits, float2& sum, uint32_t* pk) {
+            float4 v = {};
 #pragma unroll
             for (int k = 0; k < 16; ++k) {
               const float2 y = fma2(x[k], rs2, make_float2(b1, b1));
@@ -343,8 +346,8 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
               }
               if (Q8) {
                 sum = add2(sum, e);
-                const float2 v = *reinterpret_cast<const float2*>(vs + c + 2 * k);
-                e = mul2(e, mul2(v, make_float2(inv, inv)));
+                if (k % 2 == 0) v = *reinterpret_cast<const float4*>(vs + c + 2 * k);
+                e = mul2(e, k % 2 == 0 ? make_float2(v.x, v.y) : make_float2(v.z, v.w));
                 if (bits != 0xffffffffu) {
                   if (!(bits >> (2 * k) & 1u)) e.x = 0.f;
                   if (!(bits >> (2 * k + 1) & 1u)) e.y = 0.f;
@@ -398,13 +401,12 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
             const float to = mx > ref + SLACK ? mx : ref;     // by the row's own scores: rows stay independent
             float f = to == -CUDART_INF_F ? 1.f : exp2f(ref - to);
             ref = to;
-            l = mul2(l, make_float2(f, f));
-            if (Q8 && top > unit) {
-              const uint32_t e = min((__float_as_uint(top) >> 23) + 1u, 254u);
-              const float to_v = __uint_as_float(e << 23);
+            if (Q8 && top > unit) {                           // a power of two up to twice the largest scale, at most 2^127
+              const float to_v = __uint_as_float(min((__float_as_uint(top) >> 23) + 1u, 254u) << 23);
               f *= unit / to_v;
               unit = to_v;
             }
+            l = mul2(l, make_float2(f, f));
             if (items > 0 && __any_sync(0xffffffffu, f != 1.f)) {      // S of this item is behind P.V of the last one
 #pragma unroll 1
               for (int c = 0; c < D; c += 32) {
@@ -465,9 +467,8 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
         tc_fence_after();
       }
       if (!(ok = meet())) break;                            // both groups are through: queries, mask and flags are final
-      float l1 = l.x + l.y, m1 = ref == -CUDART_INF_F ? ref : ref - LIFT;
-      const float f1 = Q8 ? unit : 1.f;
-      float f0 = f1, f2 = 0.f;                              // on this group's O, on the other's
+      float l1 = l.x + l.y, m1 = ref == -CUDART_INF_F ? ref : ref - LIFT + (Q8 ? log2_of(unit) : 0.f);
+      float f0 = 1.f, f2 = 0.f;                              // on this group's O, on the other's
       if (MB == 1) {
         if (w == 1) {
           ml_s[r] = make_float2(m1, l1);
@@ -476,7 +477,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
             uint32_t v[32] = {};
             if (items > 0) { tmem_ld32(t_o + c, v); tmem_wait_ld(); }
 #pragma unroll
-            for (int k = 0; k < 32; ++k) join_s[(c + k) * 128 + r] = __uint_as_float(v[k]) * f1;
+            for (int k = 0; k < 32; ++k) join_s[(c + k) * 128 + r] = __uint_as_float(v[k]);
           }
         }
         if (!(ok = meet())) break;
@@ -485,7 +486,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
           const float m = fmaxf(m1, o.x), use = m == -CUDART_INF_F ? 0.f : m;
           const float e1 = exp2f(m1 - use);
           f2 = exp2f(o.x - use);
-          f0 = f1 * e1;
+          f0 = e1;
           l1 = fmaf(l1, e1, o.y * f2);
           m1 = m;
         }
