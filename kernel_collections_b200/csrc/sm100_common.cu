@@ -9,17 +9,16 @@ __global__ void clear_status_kernel(int* status) {
 }
 
 EncodeTiledFn get_encode() {
-  static EncodeTiledFn fn = nullptr;
-  static bool tried = false;
-  if (tried) return fn;
-  tried = true;
-  void* p = nullptr;
-  cudaDriverEntryPointQueryResult q;
-  if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
-      q == cudaDriverEntryPointSuccess)
-    fn = reinterpret_cast<EncodeTiledFn>(p);
-  else
+  // looked up once; a second thread waits for the first one's answer
+  static const EncodeTiledFn fn = []() -> EncodeTiledFn {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
+        q == cudaDriverEntryPointSuccess)
+      return reinterpret_cast<EncodeTiledFn>(p);
     cudaGetLastError();
+    return nullptr;
+  }();
   return fn;
 }
 
@@ -29,8 +28,19 @@ bool encode_tiled_16bit(CUtensorMap* m, int dtype, int rank, const void* ptr, co
   if (!fn) return false;
   cuuint32_t es[5] = {1, 1, 1, 1, 1};
   const CUtensorMapDataType dt = dtype == XKV_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
-  return fn(m, dt, (cuuint32_t)rank, const_cast<void*>(ptr), dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
-            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+  for (int again = 0; again < 2; ++again) {
+    const CUresult r = fn(m, dt, (cuuint32_t)rank, const_cast<void*>(ptr), dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                          CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r == CUDA_SUCCESS) return true;
+    // a host thread that has made no CUDA call of its own has no context yet: setting its device gives it one
+    int dev = 0;
+    if ((r != CUDA_ERROR_INVALID_CONTEXT && r != CUDA_ERROR_NOT_INITIALIZED) || cudaGetDevice(&dev) != cudaSuccess ||
+        cudaSetDevice(dev) != cudaSuccess) {
+      cudaGetLastError();
+      return false;
+    }
+  }
+  return false;
 }
 
 }  // namespace sm100

@@ -360,6 +360,42 @@ def test_another_stream_and_no_sync_between_calls():
     assert all(torch.equal(o, want) for o in outs)
 
 
+def test_two_host_threads_at_once():
+    """Calls of several shapes from two threads, on one stream and on two: none sees the other's partial results."""
+    import threading
+    cases = []
+    for i, (T, L, code) in enumerate([(1, 5000, "int8"), (9, 700, "dense"), (1, 300, "e4m3"), (30, 2000, "dense")]):
+        q, k, v, mask, _ = case(20 + i, 2, 8, 2, T, L, 128, torch.bfloat16, code, "tree")
+        want, _, _ = run(q, k, v, mask, None, code)
+        qd, kd, vd, md = q.to(DEV), k.to(DEV), v.to(DEV), mask.to(DEV)
+        if code == "dense":
+            cases.append((lambda qd=qd, kd=kd, vd=vd, md=md: K.group_query_attention_tree(qd, kd, vd, md, tcgen05=PIN), want))
+        else:
+            c = K.quantized_cache(2, 2, L, 128, code=code)
+            K.quantized_cache_append(c, kd, vd, 0)
+            cases.append((lambda qd=qd, c=c, md=md: K.group_query_attention_quantized(qd, c, md, tcgen05=PIN), want))
+    torch.cuda.synchronize()
+    wrong = []
+
+    def work(first, stream):
+        try:
+            with torch.cuda.stream(stream):
+                outs = [(n, cases[n][0]()) for i in range(60) for n in [(first + i) % len(cases)]]
+            stream.synchronize()
+            wrong.extend(n for n, o in outs if not torch.equal(o, cases[n][1]))
+        except Exception as e:      # a thread's exception is not the test's
+            wrong.append(repr(e))
+
+    for streams in ((torch.cuda.current_stream(),) * 2, (torch.cuda.Stream(), torch.cuda.Stream())):
+        # (first = 1, 3: dense caches, whose tensor maps are the threads' first CUDA calls)
+        threads = [threading.Thread(target=work, args=(2 * i + 1, s)) for i, s in enumerate(streams)]
+        for t in threads:
+            t.start()
+        for t in threads:
+            t.join()
+        assert not wrong, wrong
+
+
 def test_a_long_cache_past_32_bit_offsets():
     """The last rows of the second sequence lie past 2^31 elements."""
     KVH, D, L = 8, 128, 1_050_000
