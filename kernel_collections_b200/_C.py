@@ -284,9 +284,14 @@ def launch(fn: str, block: bytes, idx: int):
             launch(fn, block, idx)
 
 
+_status_only: dict = {}        # per device: workspace of the calls that need no more than their status words
+
+
 def run_tree_decode(block: bytes, device: torch.device, idx: int, check_status=None):
     """xkv_tree_decode with a workspace of the call's own: the caching allocator hands it on in stream order, and a
-    captured call keeps its workspace in its graph's pool, so no two graphs, streams or threads share one."""
+    captured call keeps its workspace in its graph's pool, so no two graphs, streams or threads share one.  Calls that
+    keep nothing there but status words that nobody asks for share one buffer per device (an allocation is a sixth of
+    such a call's time); made outside of captures, it lives as long as the process."""
     if idx != torch.cuda.current_device():
         with torch.cuda.device(idx):
             return run_tree_decode(block, device, idx, check_status)
@@ -295,12 +300,17 @@ def run_tree_decode(block: bytes, device: torch.device, idx: int, check_status=N
     if nbytes == 0:
         # let the entry point produce the precise status
         check(lib.xkv_tree_decode(block, None, 0, None) or -2, "xkv_tree_decode")
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
+    checked = _check_status if check_status is None else check_status
+    ws = _status_only.get(idx) if nbytes <= STATUS_BYTES and not checked else None
+    if ws is None:
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
+        if nbytes <= STATUS_BYTES and not checked and not torch.cuda.is_current_stream_capturing():
+            ws = _status_only[idx] = torch.empty(STATUS_BYTES, dtype=torch.uint8, device=device)
     stream = torch._C._cuda_getCurrentRawStream(idx)
     rc = lib.xkv_tree_decode(block, ws.data_ptr(), nbytes, stream)
     if rc:
         check(rc, "xkv_tree_decode")
-    if _check_status if check_status is None else check_status:
+    if checked:
         raise_on_status(ws.data_ptr(), stream, "xkv_tree_decode")
 
 
@@ -318,6 +328,7 @@ def last_status(device: torch.device):
 
 
 BUILTIN_SCRATCH_BYTES = 8 << 20
+STATUS_BYTES = 256      # the status words at the start of every workspace
 
 
 def run_decode_builtin_scratch(params: DecodeParams, device: torch.device):

@@ -23,8 +23,9 @@
 //    (it cancels in O / l) so that those down to 2^-20 of the largest keep all 11 bits, and the value scales are taken
 //    relative to a power of two above the largest seen.
 //  * fp32 queries: Q and P in two fp16 terms each (22 bits), two MMAs instead of one.
-// 4 x 131071 rows of 8 heads (e4m3, 8 query rows per head, 1.1 GB): 173 us, 6.4 TB/s; the same in int8, with 16 query rows or
-// with fp32 queries within 5 %.  16 ragged sequences of up to 16384 int8 rows (0.42 GB): 78 us.  One sequence of 777 rows: 15 us,
+// 4 x 131071 rows of 8 heads (e4m3, 8 query rows per head, 1.1 GB): 173 to 190 us, 5.8 to 6.4 TB/s; the same in int8, with 16 query rows or
+// with fp32 queries within 5 %.  16 ragged sequences of up to 16384 int8 rows (0.42 GB): 78 to
+// 83 us.  One sequence of 777 rows: 13 us,
 // the host's time for the call.
 #include "tree_common.cuh"
 #include "sm100_common.cuh"
