@@ -325,7 +325,8 @@ typedef enum xkv_cache_code { XKV_CACHE_DENSE = 0, XKV_CACHE_INT8 = 1, XKV_CACHE
  * of `dtype` goes to cache row start_b + t, where start_b = positions ? positions[b] : position.  With `lengths`
  * (device int32, batch entries) only the first min(lengths[b], num_tokens) tokens of sequence b are written.
  * xkv_cache_read writes code * scale of cache rows start_b + t to k / v.  Cache rows outside [0, capacity) are
- * left alone by the append and read as zeros by the read; `lengths` is the append's alone.  head_dim <= 1024.
+ * left alone by the append and read as zeros by the read; `lengths` is the append's alone.  head_dim <= 1024,
+ * batch <= 32767, num_kv_heads <= 65535.
  */
 typedef struct xkv_cache_params {
   int32_t dtype, cache_code, batch, num_kv_heads, num_tokens, capacity, head_dim;

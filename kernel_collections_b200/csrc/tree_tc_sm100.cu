@@ -15,10 +15,12 @@
 // The softmax takes one pass over S as long as no row's reference has to move (lazily, see SLACK below): weights are
 // taken against the old reference while the new maximum is formed, kept in registers, and taken again in the rare tile that
 // moves a reference or holds drafted tokens.  Number ranges (query scaling, LIFT, value scales relative to a power of two) are those of
-// tree_stream_sm100.cu.  P is rounded to the 16-bit type of the product and l sums the rounded values.
+// tree_stream_sm100.cu.  P is rounded to the 16-bit type of the product; over 16-bit caches l
+// sums the rounded values.
 // What bounds it.  Per 128 x 128 item the tensor core needs 1024 cycles and the exponentials 1024 of the 16-per-clock unit; a
 // group's chain (softmax 1800, then P.V and S with their latencies 1400) leaves about 2000 per item.  512 fp16 rows over
-// 4 x 32768 rows of 8 heads: 16-bit cache 323 us (852 TFLOP/s), int8 450 us (611: the softmax waits for scales from shared memory).  104 rows over 8 x 16384 ragged bf16 rows: 100 us, steady tiles at the rate of HBM, the rest set-up and ends of the
+// 4 x 32768 rows of 8 heads: 16-bit cache 323 us (852 TFLOP/s), int8 459 us (599: the softmax waits for scales from shared
+// memory).  104 rows over 8 x 16384 ragged bf16 rows: 100 us, steady tiles at the rate of HBM, the rest set-up and ends of the
 // strips.  Handing the exponentials from one group to the other in strict turns was measured slower (536 us against 474).
 // All waits are bounded; a group that gives up raises the abort flag, which ends the others' waits.
 #include "tree_common.cuh"

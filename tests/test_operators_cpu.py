@@ -88,6 +88,7 @@ def test_bad_parameter_blocks_are_refused_on_the_host():
                    dict(head_dim=0), dict(k=0), dict(v=0), dict(kc=0), dict(vc=0), dict(ks=0), dict(vs=0)]:
             assert fn(cache(**kw), None) == -1, kw
         assert fn(cache(head_dim=1025), None) == -2 and fn(None, None) == -1
+        assert fn(cache(batch=32768), None) == -2 and fn(cache(kv_heads=65536), None) == -2
     for kw in [dict(dtype=3), dict(code=3), dict(batch=0), dict(heads=0), dict(kv_heads=0), dict(kv_heads=3), dict(tokens=0),
                dict(kv_len=0), dict(head_dim=0), dict(splits=-1), dict(q=0), dict(k=0), dict(v=0), dict(out=0), dict(code=1),
                dict(code=2, ks=A)]:
