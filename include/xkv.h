@@ -377,6 +377,15 @@ XKV_API const char* xkv_tree_decode_plan(const xkv_tree_params* p);
 XKV_API size_t xkv_tree_decode_workspace_bytes(const xkv_tree_params* p);
 XKV_API int xkv_tree_decode(const xkv_tree_params* p, void* workspace, size_t workspace_bytes, void* stream);
 
+/*
+ * XKV_STATUS_BYTES of the library's own memory on the current device (NULL where there is none), held until the process exits: a
+ * workspace for calls that need no more than that and whose status nobody reads.  Calls on any streams and threads may
+ * use it at once: they store status words there and read nothing.  The first call on a device resolves the address
+ * (cudaGetSymbolAddress); make it outside any stream capture.
+ */
+#define XKV_STATUS_BYTES 256u
+XKV_API void* xkv_tree_status_scratch(void);
+
 #ifdef __cplusplus
 }
 #endif

@@ -31,6 +31,7 @@ EXPORTS = [
     "xkv_rope_table", "xkv_rope_query", "xkv_latent_append", "xkv_peer_allgather",
     "xkv_rotary_params_size", "xkv_rotary", "xkv_cache_params_size", "xkv_cache_append", "xkv_cache_read",
     "xkv_tree_params_size", "xkv_tree_decode_plan", "xkv_tree_decode_workspace_bytes", "xkv_tree_decode",
+    "xkv_tree_status_scratch",
 ]
 
 # Parameter blocks of the per-token operators, packed in the field order of include/xkv.h (native alignment; the sizes are
@@ -141,6 +142,8 @@ def load():
         lib.xkv_tree_decode_workspace_bytes.argtypes = [C.c_char_p]
         lib.xkv_tree_decode.restype = C.c_int
         lib.xkv_tree_decode.argtypes = [C.c_char_p, C.c_void_p, C.c_size_t, C.c_void_p]
+        lib.xkv_tree_status_scratch.restype = C.c_void_p
+        lib.xkv_tree_status_scratch.argtypes = []
         for name, block in (("xkv_rotary_params_size", ROTARY_PARAMS), ("xkv_cache_params_size", CACHE_PARAMS),
                             ("xkv_tree_params_size", TREE_PARAMS)):
             fn = getattr(lib, name)
@@ -284,14 +287,14 @@ def launch(fn: str, block: bytes, idx: int):
             launch(fn, block, idx)
 
 
-_status_only: dict = {}        # per device: workspace of the calls that need no more than their status words
+_status_scratch: dict = {}     # per device: address of the library's own status words
 
 
 def run_tree_decode(block: bytes, device: torch.device, idx: int, check_status=None):
     """xkv_tree_decode with a workspace of the call's own: the caching allocator hands it on in stream order, and a
     captured call keeps its workspace in its graph's pool, so no two graphs, streams or threads share one.  Calls that
-    keep nothing there but status words that nobody asks for share one buffer per device (an allocation is a sixth of
-    such a call's time); made outside of captures, it lives as long as the process."""
+    keep nothing there but status words that nobody asks for store them in the library's own memory instead (an allocation is
+    a sixth of such a call's time): memory that is no tensor's, before or after."""
     if idx != torch.cuda.current_device():
         with torch.cuda.device(idx):
             return run_tree_decode(block, device, idx, check_status)
@@ -301,17 +304,22 @@ def run_tree_decode(block: bytes, device: torch.device, idx: int, check_status=N
         # let the entry point produce the precise status
         check(lib.xkv_tree_decode(block, None, 0, None) or -2, "xkv_tree_decode")
     checked = _check_status if check_status is None else check_status
-    ws = _status_only.get(idx) if nbytes <= STATUS_BYTES and not checked else None
-    if ws is None:
+    ptr = None
+    if nbytes <= STATUS_BYTES and not checked:
+        ptr = _status_scratch.get(idx)
+        if ptr is None and not torch.cuda.is_current_stream_capturing():
+            ptr = lib.xkv_tree_status_scratch()
+            if ptr:
+                _status_scratch[idx] = ptr
+    if not ptr:
         ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
-        if nbytes <= STATUS_BYTES and not checked and not torch.cuda.is_current_stream_capturing():
-            ws = _status_only[idx] = torch.empty(STATUS_BYTES, dtype=torch.uint8, device=device)
+        ptr = ws.data_ptr()
     stream = torch._C._cuda_getCurrentRawStream(idx)
-    rc = lib.xkv_tree_decode(block, ws.data_ptr(), nbytes, stream)
+    rc = lib.xkv_tree_decode(block, ptr, nbytes, stream)
     if rc:
         check(rc, "xkv_tree_decode")
     if checked:
-        raise_on_status(ws.data_ptr(), stream, "xkv_tree_decode")
+        raise_on_status(ptr, stream, "xkv_tree_decode")
 
 
 def last_status(device: torch.device):

@@ -349,7 +349,7 @@ bool make_plan(const xkv_tree_params& p, TreePlan* pl) {
   if (grid > 0x3fffffff) return false;
   pl->grid = (int)grid;
   pl->merged = units > 1;
-  size_t off = 256;
+  size_t off = XKV_STATUS_BYTES;
   const size_t rows = pl->merged ? (size_t)(2 * grid) * pl->block_rows : 0;
   pl->off_o = off;
   off += align_up(rows * p.head_dim * sizeof(float), 256);
@@ -374,7 +374,16 @@ int tree_merge(const tree::Args& a, cudaStream_t st) {
 
 using namespace xkv;
 
+static __device__ __align__(256) unsigned char g_status_scratch[XKV_STATUS_BYTES];
+
 extern "C" {
+
+void* xkv_tree_status_scratch(void) {
+  void* sym = nullptr;
+  if (cudaGetSymbolAddress(&sym, g_status_scratch) == cudaSuccess) return sym;
+  cudaGetLastError();
+  return nullptr;
+}
 
 size_t xkv_tree_params_size(void) { return sizeof(xkv_tree_params); }
 

@@ -491,3 +491,26 @@ def test_status_check_passes_on_good_calls():
         check(15, 2, 8, 2, 20, 300, 128, torch.bfloat16, "int8")
     finally:
         _C.set_check_status(prev)
+
+
+def test_calls_that_need_no_scratch_leave_other_memory_alone():
+    """A device's first small call comes on a stream whose freed tensor is still being read there; a second small call on
+    another stream does not wait for it.  Neither stores anything in the tensor's memory."""
+    q, k, v, mask, _ = case(30, 1, 8, 2, 2, 60, 128, torch.bfloat16, "dense", "tree")
+    want, _, _ = run(q, k, v, mask, None, "dense", tcgen05=False)
+    qd, kd, vd, md = q.to(DEV), k.to(DEV), v.to(DEV), mask.to(DEV)
+    call = lambda: K.group_query_attention_tree(qd, kd, vd, md, tcgen05=False, check_status=False)  # noqa: E731
+    one, two = torch.cuda.Stream(), torch.cuda.Stream()
+    for nbytes in (256, 512):
+        _C._status_scratch.clear()
+        torch.cuda.synchronize()
+        with torch.cuda.stream(one):
+            x = torch.full((nbytes,), 7, dtype=torch.uint8, device=DEV)
+            torch.cuda._sleep(20_000_000)              # some 10 ms
+            y = x.clone()
+            del x
+            first = call()
+        with torch.cuda.stream(two):
+            second = call()
+        torch.cuda.synchronize()
+        assert (y == 7).all() and torch.equal(first, want) and torch.equal(second, want)

@@ -130,3 +130,12 @@ def test_kernel_selection_follows_the_call():
     assert plan(tokens=8, kv_len=100000, flags=_C.FLAG_TREE_MMA_SYNC) == b"stream"
     assert plan(tokens=4, kv_len=100000, flags=_C.FLAG_TREE_TCGEN05) == b"stream"       # 16 rows
     assert plan(tokens=257, kv_len=100000) == b"stream"
+
+
+def test_status_words_alone_need_the_library_s_own_bytes():
+    lib = _C.load()
+    short = dict(tokens=1, kv_len=100)                 # one unit of work per strip: no partial results
+    assert lib.xkv_tree_decode_workspace_bytes(tree(**short)) == _C.STATUS_BYTES
+    assert lib.xkv_tree_decode_workspace_bytes(tree(tokens=1, kv_len=100000)) > _C.STATUS_BYTES
+    text = open(_C.__file__.replace("kernel_collections_b200/_C.py", "include/xkv.h")).read()
+    assert f"#define XKV_STATUS_BYTES {_C.STATUS_BYTES}u" in text
