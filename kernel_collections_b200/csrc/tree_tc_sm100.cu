@@ -136,7 +136,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
   auto bar_vempty = [&](int s) { return bar0 + 8u * (6 + s); };
   auto bar_s = [&](int w) { return bar0 + 8u * (8 + w); };          // S of the group's next item is there
   auto bar_p = [&](int w) { return bar0 + 8u * (10 + w); };         // its P is
-  const uint32_t bar_q = bar0 + 8u * 12;                            // queries and mask of the strip are in place
+  const uint32_t bar_q = bar0 + 8u * 12;                            // queries and mask of the strip are in place, the issuer is there
   const uint32_t bar_end = bar0 + 8u * 13;                          // softmax threads meet
   volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(sm + S::MISC);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(sm + S::MISC + 4);
@@ -149,7 +149,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
       mbar_init(bar_vempty(s), 1);
     }
     for (int w = 0; w < 2; ++w) { mbar_init(bar_s(w), 1); mbar_init(bar_p(w), 4); }
-    mbar_init(bar_q, 8);
+    mbar_init(bar_q, 9);                   // the softmax warps and the issuer
     mbar_init(bar_end, 8);
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -564,6 +564,10 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
       while (ok && next_piece(a, walk, pc)) {
         const Span sp = span_of(p, pc.b);
         const int items = __shfl_sync(0xffffffffu, tiles_of(pc, sp.len), 0) * MB;
+        // The issuer arrives too, so that the softmax warps never get two strips ahead: over strips without tiles nothing else
+        // holds them, and a phase that has turned twice looks like one that has not.
+        if (lead) mbar_arrive(bar_q);
+        __syncwarp();
         if (!(ok = waits(bar_q, q_phase, 60))) break;
         q_phase ^= 1u;
         tc_fence_after();

@@ -514,3 +514,20 @@ def test_calls_that_need_no_scratch_leave_other_memory_alone():
             second = call()
         torch.cuda.synchronize()
         assert (y == 7).all() and torch.equal(first, want) and torch.equal(second, want)
+
+
+@pytest.mark.parametrize("code", CODES)
+@pytest.mark.parametrize("G,T", [(4, 8), (8, 40)])
+def test_runs_of_idle_sequences(code, G, T):
+    """Slots of a serving batch that hold nothing, one after the other within a block's share of the work: no tiles, and
+    still a row of zeros each; the sequences in between are as they are alone."""
+    b, KVH, L, D = 700, 2, 260, 64
+    lens = [0] * b
+    for i, n in ((0, 260), (5, 130), (6, 41), (350, 129), (699, 260)):
+        lens[i] = n
+    q, k, v, mask, _ = case(T, b, KVH * G, KVH, T, L, D, torch.bfloat16, code, "tree")
+    out, kd, vd = run(q, k, v, mask, lens, code, check_status=True)
+    busy = [i for i in range(b) if lens[i]]
+    idle = torch.tensor([n == 0 for n in lens], device=DEV)
+    assert (out[idle] == 0).all()
+    close(out[busy], q[busy], kd[busy], vd[busy], mask, [lens[i] for i in busy], D ** -0.5, code != "dense")
