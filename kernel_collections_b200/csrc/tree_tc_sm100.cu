@@ -436,11 +436,14 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
           // Drafted rows may be hidden from some query rows only, and 0 * NaN is NaN: elements that are not finite leave
           // the tile here and are added at the end, to the rows that see their token.
           if (!(ok = wait(bar_vfull(stage), v_parity, 51))) break;
+          // MB == 2: both groups multiply with the tile, so each cleans one half of every row, and they meet before either
+          // hands its P over (their S is issued one tile ahead: neither's MMAs wait for the other's P).
           const int at = t0 + r;
           bool hit = false;
           if (at >= sp.first) {
             constexpr uint32_t EXP = std::is_same<M, __half>::value ? 0x7c00u : 0x7f80u;
-            for (int c = 0; c < D / 8; ++c) {
+            constexpr int PIECES = D / 8 / MB;
+            for (int c = MB == 2 ? w * PIECES : 0, end = c + PIECES; c < end; ++c) {
               uint4* ad = reinterpret_cast<uint4*>(sm + S::V + stage * S::TILE + (c >> 3) * BOX + r * 128 + ((c & 7) << 4));
               uint32_t v[4] = {ad->x, ad->y, ad->z, ad->w};
               bool here = false;
@@ -456,6 +459,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
             if (hit && at >= 0 && at < sp.len) atomicOr(&bad_s[u >> 5], 1u << (u & 31));
           }
           asm volatile("fence.proxy.async.shared::cta;" ::: "memory");      // before the MMA reads the tile
+          if (MB == 2 && !(ok = meet())) break;
         }
         tc_fence_before();
         arrive(bar_p(w));

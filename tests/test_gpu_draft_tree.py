@@ -531,3 +531,44 @@ def test_runs_of_idle_sequences(code, G, T):
     idle = torch.tensor([n == 0 for n in lens], device=DEV)
     assert (out[idle] == 0).all()
     close(out[busy], q[busy], kd[busy], vd[busy], mask, [lens[i] for i in busy], D ** -0.5, code != "dense")
+
+
+def scattered(v, lens, T, kinds):
+    """`v` with one element of every drafted row replaced by one of `kinds` in turn, and the places: (sequence, drafted token,
+    column, kind)."""
+    v = v.clone()
+    places = []
+    for i, n in enumerate(lens):
+        for u in range(T):
+            if n - T + u < 0:
+                continue
+            col, kind = (7 * u + 31 * (u % 2)) % v.shape[3], kinds[u % len(kinds)]
+            v[i, :, n - T + u, col] = kind
+            places.append((i, u, col, kind))
+    return v, places
+
+
+def expected_with(clean, places, mask, T):
+    """`clean` (the output with zeros in those places) plus what each token sees of them."""
+    want = clean.cpu().clone()
+    for i, u, col, kind in places:
+        sees = (mask if mask.dim() == 2 else mask[i])[:, u]
+        want[i, :, sees, col] += torch.tensor(kind, dtype=want.dtype)
+    return want
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("G,T,D", [(4, 3, 128), (4, 8, 128), (4, 8, 64), (8, 40, 128), (8, 40, 64), (1, 250, 128)])
+def test_values_that_are_not_finite_reach_their_column_of_the_rows_that_see_them(dtype, G, T, D):
+    """Dense drafted rows, every one with a NaN or an infinity somewhere; the tree hides most from any one token."""
+    b, KVH, L = 2, 2, 300
+    lens = [300, max(T - 2, 1)]
+    q, k, v, mask, _ = case(T + D, b, KVH * G, KVH, T, L, D, dtype, "dense", "trees")
+    bad, places = scattered(v, lens, T, [float("inf"), float("nan"), -float("inf"), float("inf")])
+    zero, _ = scattered(v, lens, T, [0.0])
+    clean, _, _ = run(q, k, zero, mask, lens, "dense")
+    out, _, _ = run(q, k, bad, mask, lens, "dense")
+    want = expected_with(clean, places, mask, T)
+    out = out.cpu()
+    assert torch.equal(out.isnan(), want.isnan()) and torch.equal(out.nan_to_num(5.0, 6.0, 7.0), want.nan_to_num(5.0, 6.0, 7.0))
+    assert want.isnan().any() and want.isinf().any() and want.isfinite().any()
