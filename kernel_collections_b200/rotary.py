@@ -138,6 +138,8 @@ def rotary_embedding(query, key, inv_freq, position, *, interleaved=False, magni
             if o.shape != t.shape or o.dtype != dt or (o.stride(3) != 1 and D != 1):
                 raise ValueError("outputs must have the inputs' shapes and dtype and a contiguous last dim")
     if query.numel() == 0:
+        if key is not None and key.numel():      # no query heads: the keys turn as the call's only heads
+            rotary_embedding(key, None, inv_freq, position, interleaved=interleaved, magnitude=magnitude, out=(ko, None))
         return qo, ko
     qt, kt, kp, kop = qo.stride(), (0, 0, 0, 0), 0, 0
     if k is not None:

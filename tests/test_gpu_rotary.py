@@ -145,3 +145,17 @@ def test_rotary_refusals():
             K.rotary_embedding(**{**dict(query=q, key=k, inv_freq=f, position=0), **kw})
     with pytest.raises(RuntimeError, match="CUDA"):
         K.rotary_embedding(q.cpu(), None, f, 0)
+
+
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_keys_alone(interleaved):
+    """No query heads: the keys turn all the same, into a new tensor and into a given one."""
+    q, k = inputs(11, 2, 0, 3, 5, 64, torch.bfloat16)
+    f, _ = K.rotary_frequencies(32)
+    want = K.rotary_embedding(k, None, f, 7, interleaved=interleaved)[0]
+    qo, ko = K.rotary_embedding(q, k, f, 7, interleaved=interleaved)
+    assert qo.shape == q.shape and torch.equal(ko, want)
+    out = (torch.empty_like(q), torch.full_like(k, 3.0))
+    got = K.rotary_embedding(q, k, f, 7, interleaved=interleaved, out=out)
+    assert got[0] is out[0] and got[1] is out[1] and torch.equal(out[1], want)
+    assert K.rotary_embedding(k, q, f, 7, interleaved=interleaved)[1].shape == q.shape
