@@ -12,11 +12,10 @@
 //  * 8-bit codes are widened in registers on their way into the MMA and never written back.  The contraction index of
 //    Q.K^T may be permuted freely, so a thread takes 16 consecutive codes of a token (one 16-byte read) and Q is laid
 //    out to match.  For P.V the two tokens of an operand register are interleaved by byte permutes.  int8: the code
-//    with its sign bit flipped under the exponent byte 0x64 is the half 1024 + 128 + code; e4m3 converts in pairs.
+//    with its sign bit flipped under the exponent byte 0x64 is the half 1024 + 128 + code, less 1152 (exactly; taken off
+//    the score instead, the offset's roundings are as large as the scores of keys whose scale one channel has set); e4m3
+//    converts in pairs.
 //    Widened codes are exact in fp16 (8 significant bits), so the products run in fp16 whatever the query type.
-//  * The 1152 above the int8 keys is not subtracted from every element: the score's accumulator starts at -1152 sum(q).
-//    The partial sums are 1152 |sum q| large, an fp32 rounding of which is below 2^-17 of sum |q||code|.  (fp32
-//    queries subtract it; so do the values, whose sums run over thousands of tokens.)
 //  * Scales never touch the codes: the key scale multiplies the score, the value scale the weight.
 //  * fp16 ranges: a query row is multiplied by a power of two that brings its largest element to 2^14..2^15, and divided
 //    out of the scores in fp32: elements below 2^-28 of the largest lose bits, others none.  Weights carry the factor 2^6
@@ -91,8 +90,6 @@ __device__ __forceinline__ uint32_t widen_e4m3(uint32_t x, int high) {
   asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"(two));
   return r;
 }
-// int8 codes still 1152 above their value (sign bits flipped beforehand)
-__device__ __forceinline__ uint32_t raise_int8(uint32_t x, int high) { return __byte_perm(x, 0x64646464u, high ? 0x4342u : 0x4140u); }
 // 8 x 8 transpose of 16-bit elements across the warp
 __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
   uint32_t y;
@@ -129,7 +126,6 @@ template <typename T, int CODE, int D, int TERMS, int RB>
 __global__ void __launch_bounds__(NT, 1) stream_kernel(const Args a) {
   using S = Shape<T, CODE, D>;
   constexpr bool Q8 = CODE != XKV_CACHE_DENSE, WIDE = RB == 16;
-  constexpr bool RAISED = CODE == XKV_CACHE_INT8 && TERMS == 1;       // keys enter the product 1152 above their value
   using M = typename std::conditional<Q8, __half, typename std::conditional<std::is_same<T, float>::value, __half, T>::type>::type;
   constexpr int TOK = S::TOK, NS = TOK / 8, KS = D / 16, NO = D / 8;
   constexpr int E = WIDE ? 2 : 1;                  // tokens of every 8 that a thread scores, for each of its rows
@@ -205,7 +201,7 @@ __global__ void __launch_bounds__(NT, 1) stream_kernel(const Args a) {
     // ---- queries: scaled rows as fp32 in the free second stage, then as MMA operands --------------------------------
     float* qs = reinterpret_cast<float*>(smem + S::STAGE);                         // [row][D]
     uint4* qfrag = reinterpret_cast<uint4*>(smem + NW * STAGES * S::STAGE);        // [term][k-step / QV][lane]
-    float2* qrow = reinterpret_cast<float2*>(qfrag + TERMS * S::FRAGS / 16);       // [row]: row_scale, start of the score
+    float* qrow = reinterpret_cast<float*>(qfrag + TERMS * S::FRAGS / 16);         // [row]: row_scale
     const int T_ = p.num_tokens, G = p.num_heads / p.num_kv_heads;
     for (int r = warp; r < RB; r += NW) {
       const int row = rb * RB + r;
@@ -227,17 +223,9 @@ __global__ void __launch_bounds__(NT, 1) stream_kernel(const Args a) {
         up *= __uint_as_float((uint32_t)(e + 127) << 23);
         scale = fmaxf(scale * __uint_as_float((uint32_t)(127 - e) << 23), 1.17549435e-38f);
       }
-      float sum = 0.f;
 #pragma unroll
-      for (int i = 0; i < D / 32; ++i) {
-        x[i] *= up;
-        if (RAISED) sum += __half2float(__float2half_rn(x[i]));       // of what the product multiplies with
-        qs[r * D + i * 32 + lane] = x[i];
-      }
-      if (RAISED)
-#pragma unroll
-        for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-      if (lane == 0) qrow[r] = make_float2(scale, RAISED ? -1152.f * sum : 0.f);
+      for (int i = 0; i < D / 32; ++i) qs[r * D + i * 32 + lane] = x[i] * up;
+      if (lane == 0) qrow[r] = scale;
     }
     __syncthreads();
     for (int s = warp; s < KS; s += NW) {
@@ -259,13 +247,9 @@ __global__ void __launch_bounds__(NT, 1) stream_kernel(const Args a) {
         else reinterpret_cast<uint2*>(qfrag)[((x * KS + s) / 2 * 32 + lane) * 2 + (s & 1)] = make_uint2(f[x][0], f[x][1]);
       }
     }
-    float row_scale[2], start[2];       // score = accumulator * row_scale (* key scale), row_scale > 0
+    float row_scale[2];       // score = accumulator * row_scale (* key scale), row_scale > 0
 #pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      const float2 q = qrow[WIDE ? g + 8 * r : 2 * t + r];
-      row_scale[r] = q.x;
-      start[r] = q.y;
-    }
+    for (int r = 0; r < 2; ++r) row_scale[r] = qrow[WIDE ? g + 8 * r : 2 * t + r];
     __syncthreads();
 
     float ref[2] = {-CUDART_INF_F, -CUDART_INF_F};
@@ -313,7 +297,7 @@ __global__ void __launch_bounds__(NT, 1) stream_kernel(const Args a) {
 #pragma unroll
       for (int n = 0; n < NS * E / 2; ++n)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) sc[n][i] = start[WIDE ? i >> 1 : i & 1];
+        for (int i = 0; i < 4; ++i) sc[n][i] = 0.f;
 #pragma unroll
       for (int i = 0; i < S::CH / 4; ++i) {
         uint4 qf[TERMS][S::KPC / QV];
@@ -336,8 +320,8 @@ __global__ void __launch_bounds__(NT, 1) stream_kernel(const Args a) {
             for (int m = 0; m < 2 / E; ++m) {
               if (Q8) {
                 const uint32_t x = CODE == XKV_CACHE_INT8 ? w[m][k] ^ 0x80808080u : w[m][k];
-                f[m][0] = RAISED ? raise_int8(x, 0) : widen<CODE>(x, 0);
-                f[m][1] = RAISED ? raise_int8(x, 1) : widen<CODE>(x, 1);
+                f[m][0] = widen<CODE>(x, 0);
+                f[m][1] = widen<CODE>(x, 1);
               } else {
                 f[m][0] = w[m][(2 * k) & 3];
                 f[m][1] = w[m][(2 * k + 1) & 3];
@@ -649,7 +633,7 @@ __global__ void __launch_bounds__(NT, 1) stream_kernel(const Args a) {
 template <typename T, int CODE, int D, int TERMS, int RB>
 int launch(const Args& a, cudaStream_t st) {
   auto kern = stream_kernel<T, CODE, D, TERMS, RB>;
-  constexpr int smem = NW * STAGES * Shape<T, CODE, D>::STAGE + TERMS * Shape<T, CODE, D>::FRAGS + 16 * (int)sizeof(float2);
+  constexpr int smem = NW * STAGES * Shape<T, CODE, D>::STAGE + TERMS * Shape<T, CODE, D>::FRAGS + 16 * (int)sizeof(float);
   if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) {
     cudaGetLastError();
     return XKV_ERR_LAUNCH;

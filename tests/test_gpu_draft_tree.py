@@ -572,3 +572,22 @@ def test_values_that_are_not_finite_reach_their_column_of_the_rows_that_see_them
     out = out.cpu()
     assert torch.equal(out.isnan(), want.isnan()) and torch.equal(out.nan_to_num(5.0, 6.0, 7.0), want.nan_to_num(5.0, 6.0, 7.0))
     assert want.isnan().any() and want.isinf().any() and want.isfinite().any()
+
+
+@pytest.mark.parametrize("code", ["int8", "e4m3"])
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("G,T", [(4, 1), (4, 4), (8, 20)])
+def test_keys_with_one_large_channel(dtype, code, G, T):
+    """One channel sets the scale of every key row and the queries hardly look at it: the codes they do look at are 0 and
+    +-1, and the queries share a sign, so that an offset of the codes would add up to much more than the score."""
+    L, D = 400, 128
+    g = torch.Generator().manual_seed(T)
+    q = torch.rand(1, 2 * G, T, D, generator=g) + 0.5
+    q[..., 77] = 2.0 ** -10
+    k = 8.0 * torch.randint(-1, 2, (1, 2, L, D), generator=g).float()
+    k[..., 77] = 8.0 * 127
+    v = torch.randn(1, 2, L, D, generator=g)
+    q = q.to(dtype)
+    mask = random_tree(g, T)
+    out, kd, vd = run(q, k, v, mask, None, code)
+    close(out, q, kd, vd, mask, [L], D ** -0.5, True)
