@@ -166,6 +166,37 @@ __device__ __forceinline__ bool next_piece(const Args& a, Walk& w, Piece& pc) {
   return true;
 }
 
+// Whole powers of two, for the references of the exponents and the factors between them.
+// 2^x for a whole x up to 127; 0 below the smallest fp32 (x = -infinity included)
+__device__ __forceinline__ float pow2(float x) {
+  const int k = (int)fmaxf(x, -150.f);
+  return k >= -126 ? __uint_as_float((uint32_t)(k + 127) << 23) : k >= -149 ? __uint_as_float(1u << (k + 149)) : 0.f;
+}
+// the factor from reference `from` to `to`
+__device__ __forceinline__ float moved(float from, float to) { return from == to ? 1.f : pow2(from - to); }
+// log2 |x|, absolute error below 2^-20; -infinity for 0 and for what is not finite
+__device__ __forceinline__ float log2_size(float x) {
+  float y;
+  asm("lg2.approx.f32 %0, %1;" : "=f"(y) : "f"(fabsf(x)));
+  return y < CUDART_INF_F ? y : -CUDART_INF_F;
+}
+
+// Over 8-bit caches the product takes weight * value scale, and the reference of the exponents (a whole number) follows the
+// largest such product, not the largest scale: a row without weight takes no bits from the others, however large its values.
+// The weights and their sum l carry the same reference.  It stays within FLOOR bits below the largest score, so that they stay below
+// 2^127; above it lies at most the largest scale (up to 2^112 weights down to 2^-20 of the largest remain in fp32).
+constexpr float FLOOR = 90.f;
+constexpr float LARGEST_PRODUCT = 32768.f, LARGEST_SUM = 8.5070592e37f;      // 2^15 (fp16 ends at 65504); 2^126
+// References of pieces may lie far apart, so sums are brought to 1..2 before pieces are joined by their weights: returns the factor
+// on O and moves l and m accordingly.
+__device__ __forceinline__ float settle_sum(float& m, float& l) {
+  if (!(l > 0.f && l < CUDART_INF_F)) return 1.f;
+  const float e = (float)((int)(__float_as_uint(l) >> 23) - 127), f = pow2(-e);
+  l *= f;
+  m += e;
+  return f;
+}
+
 }  // namespace tree
 
 // ---- host side -------------------------------------------------------------------------------------------------

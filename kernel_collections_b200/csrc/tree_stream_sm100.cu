@@ -19,8 +19,8 @@
 //  * Scales never touch the codes: the key scale multiplies the score, the value scale the weight.
 //  * fp16 ranges: a query row is multiplied by a power of two that brings its largest element to 2^14..2^15, and divided
 //    out of the scores in fp32: elements below 2^-28 of the largest lose bits, others none.  Weights carry the factor 2^6
-//    (it cancels in O / l) so that those down to 2^-20 of the largest keep all 11 bits, and the value scales are taken
-//    relative to a power of two above the largest seen.
+//    (it cancels in O / l) and go into the product times their value scale, relative to the largest such product: those down
+//    to 2^-20 of it keep all 11 bits, however large the scale of a row without weight may be.
 //  * fp32 queries: Q and P in two fp16 terms each (22 bits), two MMAs instead of one.
 // 4 x 131071 rows of 8 heads (e4m3, 8 query rows per head, 1.1 GB): 173 to 190 us, 5.8 to 6.4 TB/s; the same in int8, with 16 query rows or
 // with fp32 queries within 5 %.  16 ragged sequences of up to 16384 int8 rows (0.42 GB): 78 to
@@ -252,9 +252,8 @@ __global__ void __launch_bounds__(NT, 1) stream_kernel(const Args a) {
     for (int r = 0; r < 2; ++r) row_scale[r] = qrow[WIDE ? g + 8 * r : 2 * t + r];
     __syncthreads();
 
-    float ref[2] = {-CUDART_INF_F, -CUDART_INF_F};
+    float ref[2] = {-CUDART_INF_F, -CUDART_INF_F};                        // of the scores; 8-bit caches: of the products
     float2 l[2] = {{0.f, 0.f}, {0.f, 0.f}};                               // WIDE: [row]{token}; else [0]{row}
-    float unit_v[2] = {0.f, 0.f};                                         // power of two the value scales are relative to
     // WIDE: [n]: rows g, g + 8 x columns 2t, 2t + 1 of 8 dims n.  Else [n / 2]: columns g of dims n, n + 1 x rows 2t, 2t + 1
     float o[NO * E / 2][4];
 #pragma unroll
@@ -342,7 +341,7 @@ __global__ void __launch_bounds__(NT, 1) stream_kernel(const Args a) {
         }
       }
       auto score = [&](int n, int r, int e) -> float& { return WIDE ? sc[n][2 * r + e] : sc[n / 2][2 * (n & 1) + r]; };
-      // ---- key scales, hidden tokens, maximum (scores still without row_scale) --------------------------------------
+      // ---- key scales and hidden tokens (scores still without row_scale) -------------------------------------------------
       uint32_t vis[2] = {0xffffffffu, 0xffffffffu};        // bit E n + e: row sees token 8n + tok0 + e
       if (Q8) {
 #pragma unroll
@@ -375,104 +374,117 @@ __global__ void __launch_bounds__(NT, 1) stream_kernel(const Args a) {
             }
         }
       }
-      float mx[2] = {-CUDART_INF_F, -CUDART_INF_F};
-      bool move = false;
-#pragma unroll
-      for (int r = 0; r < 2; ++r) {
-#pragma unroll
-        for (int n = 0; n < NS; ++n)
-#pragma unroll
-          for (int e = 0; e < E; ++e) mx[r] = fmaxf(mx[r], score(n, r, e));
-        mx[r] = across(mx[r]) * row_scale[r];
-        move |= mx[r] > ref[r] + SLACK;
-      }
-      // the value scales' common power of two: above the largest finite one that a row sees
-      float top[2] = {0.f, 0.f};
-      if (Q8 && plain) {
-        uint32_t m = 0;
-#pragma unroll
-        for (int i = 0; i < TOK; i += 32) {
-          const uint32_t v = __float_as_uint(kss[TOK + i + lane]) & 0x7fffffffu;     // magnitudes order as integers
-          m = max(m, v < 0x7f800000u ? v : 0u);
-        }
-        top[0] = top[1] = __uint_as_float(__reduce_max_sync(0xffffffffu, m));
-      } else if (Q8) {
+      // the largest score of each row of the thread in this tile, over all lanes that share the row
+      auto largest = [&](float (&mx)[2]) {
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
+          mx[r] = -CUDART_INF_F;
 #pragma unroll
           for (int n = 0; n < NS; ++n)
 #pragma unroll
-            for (int e = 0; e < E; ++e) {
-              const float v = fabsf(kss[TOK + n * 8 + tok0 + e]);
-              if (v < CUDART_INF_F && (vis[r] >> (E * n + e) & 1)) top[r] = fmaxf(top[r], v);
-            }
-          top[r] = across(top[r]);
+            for (int e = 0; e < E; ++e) mx[r] = fmaxf(mx[r], score(n, r, e));
+          mx[r] = across(mx[r]) * row_scale[r];
         }
-      }
-      if (Q8) move |= top[0] > unit_v[0] || top[1] > unit_v[1];
-      if (__any_sync(0xffffffffu, move)) {
-        float f[2];
-#pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          const float to = mx[r] > ref[r] + SLACK ? mx[r] : ref[r];      // by the row's own scores: rows stay independent
-          f[r] = to == -CUDART_INF_F ? 1.f : exp2f(ref[r] - to);
-          ref[r] = to;
-          if (WIDE) l[r] = mul2(l[r], make_float2(f[r], f[r]));
-          else if (r == 1) l[0] = mul2(l[0], make_float2(f[0], f[1]));
-        }
+      };
+      // to new references (by a row's own scores: rows stay independent), by the factors f
+      auto rescale = [&](const float (&f)[2]) {
 #pragma unroll
         for (int r = 0; r < 2; ++r)
-          if (Q8 && top[r] > unit_v[r]) {
-            // a power of two up to twice the largest scale (capped at 2^127); both are powers of two: the ratio is exact
-            const uint32_t e = min((__float_as_uint(top[r]) >> 23) + 1u, 254u);
-            const float to = __uint_as_float(e << 23);
-            f[r] *= unit_v[r] / to;
-            unit_v[r] = to;
-          }
+          if (WIDE) l[r] = mul2(l[r], make_float2(f[r], f[r]));
+        if (!WIDE) l[0] = mul2(l[0], make_float2(f[0], f[1]));
 #pragma unroll
         for (int n = 0; n < NO * E / 2; ++n)
 #pragma unroll
           for (int i = 0; i < 4; ++i) o[n][i] *= f[WIDE ? i >> 1 : i & 1];
-      }
-      // ---- weights ------------------------------------------------------------------------------------------------
-      // pf as operands of P.V: WIDE [term][n][r] tokens 8n + 2t, + 1 of row g + 8r; else [term][n][0] the same of row g
-      uint32_t pf[TERMS][NS][E];
-      {
-        float base[2], inv[2];
+      };
+      // weights of tile n: WIDE: a row's two tokens; else a token's two rows
+      auto weight = [&](int n, int r) {
+        const float* s2 = WIDE ? &sc[n][2 * r] : &sc[n / 2][2 * (n & 1)];
+        auto two = [&](auto of) { return WIDE ? make_float2(of(r), of(r)) : make_float2(of(0), of(1)); };
+        const float2 x = fma2(make_float2(s2[0], s2[1]), two([&](int i) { return row_scale[i]; }),
+                              two([&](int i) { return ref[i] == -CUDART_INF_F ? 0.f : LIFT - ref[i]; }));
+        return make_float2(ex2(x.x), ex2(x.y));
+      };
+      float2 pw[NS][E];            // what P.V multiplies with
+      if constexpr (Q8) {
+        // The products are formed against the reference as it is and show by themselves whether it has to move: few do.
+#pragma unroll 1
+        for (bool again = false;; again = true) {
+          float2 sum[2] = {l[0], l[1]};
+          float top = 0.f;
 #pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          base[r] = ref[r] == -CUDART_INF_F ? 0.f : LIFT - ref[r];
-          inv[r] = Q8 ? (unit_v[r] > 0.f ? 1.f / unit_v[r] : 0.f) : 1.f;
-        }
+          for (int n = 0; n < NS; ++n)
 #pragma unroll
-        for (int n = 0; n < NS; ++n)
-#pragma unroll
-          for (int r = 0; r < E; ++r) {          // WIDE: a row's two tokens; else a token's two rows
-            const float* s2 = WIDE ? &sc[n][2 * r] : &sc[n / 2][2 * (n & 1)];
-            const float2 scale = WIDE ? make_float2(row_scale[r], row_scale[r]) : make_float2(row_scale[0], row_scale[1]);
-            const float2 x = fma2(make_float2(s2[0], s2[1]), scale, WIDE ? make_float2(base[r], base[r]) : make_float2(base[0], base[1]));
-            float2 w = make_float2(ex2(x.x), ex2(x.y));
-            if (Q8) {
-              l[r] = add2(l[r], w);
-              float2 v;
+            for (int r = 0; r < E; ++r) {
+              float2 w = weight(n, r), v;
+              sum[r] = add2(sum[r], w);
               if (WIDE) v = *reinterpret_cast<const float2*>(kss + TOK + n * 8 + tok0);
               else v.x = v.y = kss[TOK + n * 8 + tok0];
-              w = mul2(w, mul2(v, WIDE ? make_float2(inv[r], inv[r]) : make_float2(inv[0], inv[1])));
+              w = mul2(w, v);
               if (!plain) {                    // a hidden token's scale may be anything
                 if (!(vis[WIDE ? r : 0] >> (E * n) & 1)) w.x = 0.f;
                 if (!(vis[WIDE ? r : 1] >> (E * n + E - 1) & 1)) w.y = 0.f;
               }
+              top = fmaxf(top, fmaxf(fabsf(w.x), fabsf(w.y)));
+              pw[n][r] = w;
             }
-            const uint32_t hi = TypeTraits<M>::pack2(w.x, w.y);
-            const float2 f = TypeTraits<M>::unpack2(hi);
-            if (!Q8) l[r] = add2(l[r], f);      // the sum of what P.V multiplies with: the rounding cancels
-            pf[0][n][r] = WIDE ? hi : transpose8(hi);
-            if (TERMS == 2) {
-              const uint32_t lo = TypeTraits<M>::pack2(w.x - f.x, w.y - f.y);
-              pf[TERMS - 1][n][r] = WIDE ? lo : transpose8(lo);
-            }
+          bool move = top > LARGEST_PRODUCT || ref[0] == -CUDART_INF_F || ref[1] == -CUDART_INF_F;
+#pragma unroll
+          for (int r = 0; r < E; ++r) move |= fmaxf(sum[r].x, sum[r].y) >= LARGEST_SUM;
+          if (again || !__any_sync(0xffffffffu, move)) {
+            l[0] = sum[0];
+            l[1] = sum[1];
+            break;
           }
+          float mx[2], f[2];
+          largest(mx);
+#pragma unroll
+          for (int r = 0; r < 2; ++r) {
+            float px = -CUDART_INF_F;          // the largest score + log2 |value scale|; hidden tokens' scores are -infinity
+#pragma unroll
+            for (int n = 0; n < NS; ++n)
+#pragma unroll
+              for (int e = 0; e < E; ++e) px = fmaxf(px, fmaf(score(n, r, e), row_scale[r], log2_size(kss[TOK + n * 8 + tok0 + e])));
+            px = ceilf(fmaxf(across(px), mx[r] - FLOOR));
+            const float to = px > ref[r] + SLACK ? px : ref[r];
+            f[r] = moved(ref[r], to);
+            ref[r] = to;
+          }
+          rescale(f);
+        }
+      } else {
+        float mx[2], f[2];
+        largest(mx);
+        if (__any_sync(0xffffffffu, mx[0] > ref[0] + SLACK || mx[1] > ref[1] + SLACK)) {
+#pragma unroll
+          for (int r = 0; r < 2; ++r) {
+            const float to = mx[r] > ref[r] + SLACK ? mx[r] : ref[r];
+            f[r] = to == -CUDART_INF_F ? 1.f : exp2f(ref[r] - to);
+            ref[r] = to;
+          }
+          rescale(f);
+        }
+#pragma unroll
+        for (int n = 0; n < NS; ++n)
+#pragma unroll
+          for (int r = 0; r < E; ++r) pw[n][r] = weight(n, r);
       }
+      // ---- as operands: WIDE [term][n][r] tokens 8n + 2t, + 1 of row g + 8r; else [term][n][0] the same of row g --------------
+      uint32_t pf[TERMS][NS][E];
+#pragma unroll
+      for (int n = 0; n < NS; ++n)
+#pragma unroll
+        for (int r = 0; r < E; ++r) {
+          const float2 w = pw[n][r];
+          const uint32_t hi = TypeTraits<M>::pack2(w.x, w.y);
+          const float2 f = TypeTraits<M>::unpack2(hi);
+          if (!Q8) l[r] = add2(l[r], f);      // the sum of what P.V multiplies with: the rounding cancels
+          pf[0][n][r] = WIDE ? hi : transpose8(hi);
+          if (TERMS == 2) {
+            const uint32_t lo = TypeTraits<M>::pack2(w.x - f.x, w.y - f.y);
+            pf[TERMS - 1][n][r] = WIDE ? lo : transpose8(lo);
+          }
+        }
       // Drafted rows may be hidden from some query rows only, and 0 * NaN is NaN: elements that are not finite are taken
       // out of the value tile here and added after the product, to the rows that see their token.
       uint64_t bad = 0;
@@ -584,19 +596,20 @@ __global__ void __launch_bounds__(NT, 1) stream_kernel(const Args a) {
     float* acc = reinterpret_cast<float*>(smem);               // [warp][row][OS]
     float2* ml = reinterpret_cast<float2*>(qfrag);             // [warp][row]
     static_assert(NW * RB * OS * 4 <= NW * STAGES * S::STAGE, "the ring holds the partial outputs");
+    float f_o[2];
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      float sum = WIDE ? l[r].x + l[r].y : r ? l[0].y : l[0].x, m = ref[r] == -CUDART_INF_F ? ref[r] : ref[r] - LIFT;
+#pragma unroll
+      for (int o = WIDE ? 1 : 4; o < (WIDE ? 4 : 32); o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      f_o[r] = Q8 ? settle_sum(m, sum) : 1.f;
+      if ((WIDE ? t : g) == 0) ml[warp * RB + (WIDE ? g + 8 * r : 2 * t + r)] = make_float2(m, sum);
+    }
 #pragma unroll
     for (int n = 0; n < NO * E / 2; ++n)
 #pragma unroll
       for (int i = 0; i < 4; ++i)
-        acc[(warp * RB + row_of(i)) * OS + dim_of(n, i)] = o[n][i] * (Q8 ? unit_v[WIDE ? i >> 1 : i & 1] : 1.f);
-#pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      float sum = WIDE ? l[r].x + l[r].y : r ? l[0].y : l[0].x;
-#pragma unroll
-      for (int o = WIDE ? 1 : 4; o < (WIDE ? 4 : 32); o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-      if ((WIDE ? t : g) == 0)
-        ml[warp * RB + (WIDE ? g + 8 * r : 2 * t + r)] = make_float2(ref[r] == -CUDART_INF_F ? ref[r] : ref[r] - LIFT, sum);
-    }
+        acc[(warp * RB + row_of(i)) * OS + dim_of(n, i)] = Q8 ? o[n][i] * f_o[WIDE ? i >> 1 : i & 1] : o[n][i];
     __syncthreads();
     const int live = min(RB, a.rows - rb * RB);
     for (int i = threadIdx.x; i < live * (D / 4); i += NT) {

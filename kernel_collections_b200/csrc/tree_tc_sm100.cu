@@ -14,7 +14,7 @@
 //   them to fp16 (exact) and store them in the layout that TMA would have made; scales go to the softmax threads.
 // The softmax takes one pass over S as long as no row's reference has to move (lazily, see SLACK below): weights are
 // taken against the old reference while the new maximum is formed, kept in registers, and taken again in the rare tile that
-// moves a reference or holds drafted tokens.  Number ranges (query scaling, LIFT, value scales relative to a power of two) are those of
+// moves a reference or holds drafted tokens.  Number ranges (query scaling, LIFT, products with the value scales) are those of
 // tree_stream_sm100.cu.  P is rounded to the 16-bit type of the product; over 16-bit caches l
 // sums the rounded values.
 // What bounds it.  Per 128 x 128 item the tensor core needs 1024 cycles and the exponentials 1024 of the 16-per-clock unit; a
@@ -49,8 +49,8 @@ struct Smem {
   static constexpr int Q = 0;                                   // two row blocks (the second also takes part in the join)
   static constexpr int K = Q + 2 * TILE;
   static constexpr int V = K + STAGES * TILE;
-  static constexpr int SCALES = V + STAGES * TILE;              // [stage]{key scales, value scales}[128], [stage] the wideners' largest
-  static constexpr int MASK = SCALES + STAGES * (2 * TK + WIDENERS) * 4;   // [token][words]
+  static constexpr int SCALES = V + STAGES * TILE;              // [stage]{key scales, value scales, log2 of these}[128]
+  static constexpr int MASK = SCALES + STAGES * 3 * TK * 4;   // [token][words]
   static constexpr int BAD = MASK + MAX_T * (MAX_T / 32) * 4;   // drafted tokens with values that are not finite
   static constexpr int ML = BAD + MAX_T / 32 * 4;               // [128] of the second group, MB == 1
   static constexpr int SCALE = ML + TK * 8;                     // [row] of the strip: factor on its scores
@@ -85,11 +85,6 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
 }
 template <typename T> __device__ __forceinline__ float to_float(T v) { return TypeTraits<T>::to_f(v); }
 template <typename T> __device__ __forceinline__ T from_float(float v) { return TypeTraits<T>::from_f(v); }
-
-// The value scales are taken relative to a power of two above the largest seen, at least this one (weights divided by it, and
-// their sums, stay below 2^127).  The division is part of the exponent, and O and l carry it alike.
-constexpr float SMALLEST_UNIT = 8.0779357e-28f;      // 2^-90
-__device__ __forceinline__ float log2_of(float power_of_two) { return (float)((int)(__float_as_uint(power_of_two) >> 23) - 127); }
 
 // one lane of the warp, the same one every time
 __device__ __forceinline__ bool elect() {
@@ -290,24 +285,20 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
         q_phase ^= 1u;
         if (busy) row_scale = scale_s[blk * 128 + r];
       }
-      float ref = -CUDART_INF_F, unit = SMALLEST_UNIT;       // unit: the power of two that the value scales are relative to
+      float ref = -CUDART_INF_F;                             // of the scores; over 8-bit caches of score + log2 |value scale|
       float2 l = make_float2(0.f, 0.f);
       int items = 0;
       for (int i = MB == 2 ? 0 : w; i < ntiles; i += MB == 2 ? 1 : 2, ++items) {
         const int t0 = (pc.begin + i) * TK;
         const int stage = (tiles_seen + i) % STAGES;
         const uint32_t v_parity = (uint32_t)((tiles_seen + i) / STAGES) & 1u;
-        const float* ks = reinterpret_cast<const float*>(sm + S::SCALES + stage * (2 * TK + WIDENERS) * 4);
+        const float* ks = reinterpret_cast<const float*>(sm + S::SCALES + stage * 3 * TK * 4);
         const float* vs = ks + TK;
         if (Q8 && !(ok = wait(bar_vfull(stage), v_parity, 51))) break;       // the scales come with the values
         if (!(ok = wait(bar_s(w), s_phase, 52))) break;
         s_phase ^= 1u;
         tc_fence_after();
         const bool plain = t0 + TK <= sp.first;
-        float tile_top = 0.f;
-        if (Q8)
-#pragma unroll
-          for (int k = 0; k < WIDENERS; ++k) tile_top = fmaxf(tile_top, vs[TK + k]);
         // tokens c .. c + 31 of the tile that this row sees: all in front of the drafted ones, then by the mask's bits
         auto seen = [&](int c) -> uint32_t {
           const int u0 = t0 + c - sp.first, k = u0 >> 5;          // drafted token of the first one
@@ -332,10 +323,10 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
               }
             }
           };
-          float b1;                                           // weights are 2^(score + b1), over 8-bit caches divided by unit
-          auto settle = [&]() { b1 = ref == -CUDART_INF_F ? 0.f : LIFT - ref - (Q8 ? log2_of(unit) : 0.f); };
+          float b1;                                           // weights are 2^(score + b1)
+          auto settle = [&]() { b1 = ref == -CUDART_INF_F ? 0.f : LIFT - ref; };
           settle();
-          // their weights against the reference, packed, and the sum of them
+          // their weights against the reference (over 8-bit caches times the value scales), packed, and the sum of them
           auto weights = [&](int c, const float2 (&x)[16], uint32_t bits, float2& sum, uint32_t* pk) {
             float4 v = {};
 #pragma unroll
@@ -361,19 +352,33 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
           };
           float mx = -CUDART_INF_F;
           bool done = false, known = false;                   // the row's maximum is known
-          if (__all_sync(0xffffffffu, plain && tile_top <= unit && ref > -CUDART_INF_F)) {
+          if (__all_sync(0xffffffffu, plain && ref > -CUDART_INF_F)) {
             uint32_t pk[2][32];
             float2 sum = l;
 #pragma unroll
             for (int c = 0; c < TK; c += 32) {
               float2 x[16];
               scores(c, x);
+              if (!Q8)
 #pragma unroll
-              for (int k = 0; k < 16; ++k) mx = fmaxf(mx, fmaxf(x[k].x, x[k].y));
+                for (int k = 0; k < 16; ++k) mx = fmaxf(mx, fmaxf(x[k].x, x[k].y));
               weights(c, x, 0xffffffffu, sum, pk[c / 64] + (c & 32) / 2);
             }
-            done = __all_sync(0xffffffffu, mx * row_scale <= ref + SLACK);
-            known = true;
+            bool good;
+            if (Q8) {                                         // the products show by themselves whether the reference has to move
+              __half2 top[4];
+#pragma unroll
+              for (int k = 0; k < 64; ++k) {
+                const __half2 y = __habs2(*reinterpret_cast<const __half2*>(&pk[k / 32][k & 31]));
+                top[k & 3] = k < 4 ? y : __hmax2(top[k & 3], y);
+              }
+              const float2 t = __half22float2(__hmax2(__hmax2(top[0], top[1]), __hmax2(top[2], top[3])));
+              good = fmaxf(t.x, t.y) <= LARGEST_PRODUCT && !(fmaxf(sum.x, sum.y) >= LARGEST_SUM);
+            } else {
+              good = mx * row_scale <= ref + SLACK;
+            }
+            done = __all_sync(0xffffffffu, good);
+            known = !Q8;
             if (done) {
               l = sum;
               tmem_st32(t_s, pk[0]);
@@ -381,7 +386,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
             }
           }
           if (!done) {                                        // S is still there: P has not been stored
-            float top = plain ? tile_top : 0.f;
+            float px = -CUDART_INF_F;                         // the largest score + log2 |value scale|
 #pragma unroll 1
             for (int c = 0; c < TK && !known; c += 32) {
               float2 x[16];
@@ -392,22 +397,18 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
                 const uint32_t two = bits >> (2 * k);
                 if (two & 1u) mx = fmaxf(mx, x[k].x);
                 if (two & 2u) mx = fmaxf(mx, x[k].y);
-                if (Q8 && !plain) {
-                  const float2 v = *reinterpret_cast<const float2*>(vs + c + 2 * k);
-                  if ((two & 1u) && fabsf(v.x) < CUDART_INF_F) top = fmaxf(top, fabsf(v.x));
-                  if ((two & 2u) && fabsf(v.y) < CUDART_INF_F) top = fmaxf(top, fabsf(v.y));
+                if (Q8) {
+                  const float2 v = *reinterpret_cast<const float2*>(vs + TK + c + 2 * k);
+                  if (two & 1u) px = fmaxf(px, fmaf(x[k].x, row_scale, v.x));
+                  if (two & 2u) px = fmaxf(px, fmaf(x[k].y, row_scale, v.y));
                 }
               }
             }
             mx *= row_scale;
+            if (Q8) mx = ceilf(fmaxf(px, mx - FLOOR));
             const float to = mx > ref + SLACK ? mx : ref;     // by the row's own scores: rows stay independent
-            float f = to == -CUDART_INF_F ? 1.f : exp2f(ref - to);
+            const float f = Q8 ? moved(ref, to) : to == -CUDART_INF_F ? 1.f : exp2f(ref - to);
             ref = to;
-            if (Q8 && top > unit) {                           // a power of two up to twice the largest scale, at most 2^127
-              const float to_v = __uint_as_float(min((__float_as_uint(top) >> 23) + 1u, 254u) << 23);
-              f *= unit / to_v;
-              unit = to_v;
-            }
             l = mul2(l, make_float2(f, f));
             if (items > 0 && __any_sync(0xffffffffu, f != 1.f)) {      // S of this item is behind P.V of the last one
 #pragma unroll 1
@@ -473,8 +474,9 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
         tc_fence_after();
       }
       if (!(ok = meet())) break;                            // both groups are through: queries, mask and flags are final
-      float l1 = l.x + l.y, m1 = ref == -CUDART_INF_F ? ref : ref - LIFT + (Q8 ? log2_of(unit) : 0.f);
+      float l1 = l.x + l.y, m1 = ref == -CUDART_INF_F ? ref : ref - LIFT;
       float f0 = 1.f, f2 = 0.f;                              // on this group's O, on the other's
+      if (Q8) f0 = settle_sum(m1, l1);
       if (MB == 1) {
         if (w == 1) {
           ml_s[r] = make_float2(m1, l1);
@@ -483,7 +485,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
             uint32_t v[32] = {};
             if (items > 0) { tmem_ld32(t_o + c, v); tmem_wait_ld(); }
 #pragma unroll
-            for (int k = 0; k < 32; ++k) join_s[(c + k) * 128 + r] = __uint_as_float(v[k]);
+            for (int k = 0; k < 32; ++k) join_s[(c + k) * 128 + r] = __uint_as_float(v[k]) * f0;
           }
         }
         if (!(ok = meet())) break;
@@ -492,7 +494,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
           const float m = fmaxf(m1, o.x), use = m == -CUDART_INF_F ? 0.f : m;
           const float e1 = exp2f(m1 - use);
           f2 = exp2f(o.x - use);
-          f0 = e1;
+          f0 *= e1;
           l1 = fmaf(l1, e1, o.y * f2);
           m1 = m;
         }
@@ -702,7 +704,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
       for (int i = 0; i < ntiles; ++i, ++seen) {
         const int stage = seen % STAGES;
         const uint32_t parity = ((uint32_t)(seen / STAGES) & 1u) ^ 1u;
-        float* ks = reinterpret_cast<float*>(sm + S::SCALES + stage * (2 * TK + WIDENERS) * 4);
+        float* ks = reinterpret_cast<float*>(sm + S::SCALES + stage * 3 * TK * 4);
         if (!(ok = wait(bar_kempty(stage), parity, 70))) break;
         store(kr, S::K + stage * S::TILE);
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -735,10 +737,8 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
         if (lane < ROWS) {
           ks[c4 * ROWS + lane] = k_scale;
           ks[TK + c4 * ROWS + lane] = v_scale;
+          ks[2 * TK + c4 * ROWS + lane] = log2_size(v_scale);
         }
-        const uint32_t mag = __float_as_uint(v_scale) & 0x7fffffffu;
-        const uint32_t top = __reduce_max_sync(0xffffffffu, mag < 0x7f800000u ? mag : 0u);
-        if (lane == 0) ks[2 * TK + c4] = __uint_as_float(top);
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncwarp();
         if (lane == 0) mbar_arrive(bar_vfull(stage));

@@ -9,6 +9,8 @@ Tolerance per output element.  With w the softmax weights and A = sum w |v| (64 
                            halves and for the logits' change of base, 2^-21 for the exponential
   2 (L + 8) 2^-24 A        fp32 sums over L tokens, numerator and denominator
 and 2^-25 where fp16 is subnormal."""
+import math
+
 import pytest
 import torch
 
@@ -591,3 +593,66 @@ def test_keys_with_one_large_channel(dtype, code, G, T):
     mask = random_tree(g, T)
     out, kd, vd = run(q, k, v, mask, None, code)
     close(out, q, kd, vd, mask, [L], D ** -0.5, True)
+
+
+def weighed(seed, G, T, L, low, dtype):
+    """Queries and keys whose scores are ordinary but for the rows `low`, which lie that many bits (log2) below.  The
+    offset is a channel of its own: 1 in every query, negative in those keys."""
+    D = 128
+    g = torch.Generator().manual_seed(seed)
+    q = torch.randn(1, 2 * G, T, D, generator=g)
+    k = torch.randn(1, 2, L, D, generator=g) * 0.3
+    v = torch.randn(1, 2, L, D, generator=g)
+    q[..., 0], k[..., 0] = 1.0, 0.0
+    for row, bits in low.items():
+        k[:, :, row] = 0.0
+        k[:, :, row, 0] = -bits * math.log(2.0) * D ** 0.5
+    return q.to(dtype), k, v, random_tree(g, T)
+
+
+@pytest.mark.parametrize("code", ["int8", "e4m3"])
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("G,T", [(4, 1), (4, 4), (4, 8), (8, 20)])
+@pytest.mark.parametrize("L", [60, 700])
+@pytest.mark.parametrize("bits,size", [(60, 24), (60, 32), (100, 60)])
+def test_large_values_that_carry_no_weight_take_no_bits(dtype, code, G, T, L, bits, size):
+    """Rows whose values are 2^size times the others' and whose weights are 2^-bits: all others keep their precision."""
+    at = [0, 17, L // 2]
+    q, k, v, mask = weighed(bits + T, G, T, L, {i: bits for i in at}, dtype)
+    for i in at:
+        v[:, :, i] *= 2.0 ** size
+    out, kd, vd = run(q, k, v, mask, None, code)
+    close(out, q, kd, vd, mask, [L], 128 ** -0.5, True)
+
+
+@pytest.mark.parametrize("code", ["int8", "e4m3"])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("G,T", [(4, 1), (4, 4), (4, 8), (8, 20)])
+@pytest.mark.parametrize("size", [-60, -110])
+def test_small_values_that_carry_all_the_weight(dtype, code, G, T, size):
+    """One row takes all the weight and its values are 2^size of the others', whose weights are near 2^-40: what they add
+    is most of the output.  Then the row's values are zeros."""
+    L = 300
+    q, k, v, mask = weighed(T, G, T, L, {i: 40 for i in range(L) if i != 5}, dtype)
+    for factor in (2.0 ** size, 0.0):
+        x = v.clone()
+        x[:, :, 5] *= factor
+        out, kd, vd = run(q, k, x, mask, None, code)
+        close(out, q, kd, vd, mask, [L], 128 ** -0.5, True)
+        assert (out != 0).any()
+
+
+@pytest.mark.parametrize("code", ["int8", "e4m3"])
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("G,T", [(4, 1), (4, 4), (4, 8), (8, 20)])
+def test_rows_of_zeros_before_and_between_values(dtype, code, G, T):
+    """Value rows of zeros have no scale to be relative to: first all of them, then the first 300, then every second."""
+    L = 500
+    q, k, v, mask = weighed(T, G, T, L, {}, dtype)
+    out, _, _ = run(q, k, v * 0.0, mask, None, code)
+    assert (out == 0).all()
+    for zeros in (slice(0, 300), slice(0, L, 2)):
+        x = v.clone()
+        x[:, :, zeros] = 0.0
+        out, kd, vd = run(q, k, x, mask, None, code)
+        close(out, q, kd, vd, mask, [L], 128 ** -0.5, True)
