@@ -112,6 +112,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
   constexpr bool Q8 = CODE != XKV_CACHE_DENSE;
   using M = typename std::conditional<Q8, __half, T>::type;
   using S = Smem<D, MB>;
+  constexpr bool CLEANS = CODE != XKV_CACHE_INT8;      // values may be infinite (16-bit) or NaN (16-bit, e4m3 codes 0x7f and 0xff)
   // weights are 2^(score - reference + LIFT); the reference follows the maximum when it is passed by more than SLACK
   // (fp16: below 2^15 always, and all 11 bits down to 2^-20 of the reference; bf16 has the range of fp32, and stays below 2^8
   // so that products with large values do)
@@ -433,10 +434,10 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
           }
           tmem_wait_st();
         }
-        if (!Q8 && !plain) {
+        if (CLEANS && !plain) {
           // Drafted rows may be hidden from some query rows only, and 0 * NaN is NaN: elements that are not finite leave
           // the tile here and are added at the end, to the rows that see their token.
-          if (!(ok = wait(bar_vfull(stage), v_parity, 51))) break;
+          if (!Q8 && !(ok = wait(bar_vfull(stage), v_parity, 51))) break;
           // MB == 2: both groups multiply with the tile, so each cleans one half of every row, and they meet before either
           // hands its P over (their S is issued one tile ahead: neither's MMAs wait for the other's P).
           const int at = t0 + r;
@@ -502,7 +503,7 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
       if ((MB == 2 || w == 0) && busy) {
         const float inv = !pc.whole ? 1.f : l1 == 0.f ? 0.f : 1.f / l1;
         uint32_t any_bad = 0;
-        if (!Q8)
+        if (CLEANS)
           for (int k = 0; k < words; ++k) any_bad |= bad_s[k];
 #pragma unroll 1
         for (int c = 0; c < D; c += 32) {
@@ -517,10 +518,11 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
           if (any_bad && live) {
             for (int u = 0; u < T_; ++u)
               if ((bad_s[u >> 5] >> (u & 31) & 1u) && (mask_s[tok * words + (u >> 5)] >> (u & 31) & 1u)) {
-                const T* vr = static_cast<const T*>(p.v) + (int64_t)pc.b * p.v_sb + (int64_t)pc.h * p.v_sh + (int64_t)(sp.first + u) * p.v_sl + c;
+                const int64_t vr = (int64_t)pc.b * p.v_sb + (int64_t)pc.h * p.v_sh + (int64_t)(sp.first + u) * p.v_sl + c;
 #pragma unroll
                 for (int k = 0; k < 32; ++k) {
-                  const float y = to_float(vr[k]);
+                  const float y = Q8 ? __half2float(__half(__nv_cvt_fp8_to_halfraw(static_cast<const uint8_t*>(p.v)[vr + k], __NV_E4M3)))
+                                     : to_float(static_cast<const T*>(p.v)[vr + k]);
                   if (!(fabsf(y) < CUDART_INF_F)) x[k] += y;
                 }
               }
@@ -713,31 +715,11 @@ tree_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ 
         const float k_scale = ksr;
         if (i + 1 < ntiles) load_k(i + 1);
         if (!(ok = wait(bar_vempty(stage), parity, 71))) break;
-        const int at0 = (pc.begin + i) * TK + c4 * ROWS;
-        float v_scale = vsr;
-        if (CODE == XKV_CACHE_E4M3 && at0 + ROWS > sp.first) {
-          // a NaN code among the drafted rows would reach rows that do not see it: the code becomes zero and the row's
-          // scale the NaN, which the weights of hidden tokens leave out
-          uint32_t bad = 0;
-#pragma unroll
-          for (int k = 0; k < N; ++k) {
-            uint32_t* v = reinterpret_cast<uint32_t*>(&vr[k]);
-            bool here = false;
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-#pragma unroll
-              for (int e = 0; e < 32; e += 8)
-                if ((v[j] >> e & 0x7fu) == 0x7fu && at0 + k * RPI + r0 >= sp.first) { v[j] &= ~(0xffu << e); here = true; }
-            if (here) bad |= 1u << (k * RPI + r0);
-          }
-          bad = __reduce_or_sync(0xffffffffu, bad);
-          if (bad >> lane & 1u) v_scale = CUDART_NAN_F;
-        }
         store(vr, S::V + stage * S::TILE);
         if (lane < ROWS) {
           ks[c4 * ROWS + lane] = k_scale;
-          ks[TK + c4 * ROWS + lane] = v_scale;
-          ks[2 * TK + c4 * ROWS + lane] = log2_size(v_scale);
+          ks[TK + c4 * ROWS + lane] = vsr;
+          ks[2 * TK + c4 * ROWS + lane] = log2_size(vsr);
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncwarp();

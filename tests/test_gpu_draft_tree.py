@@ -656,3 +656,36 @@ def test_rows_of_zeros_before_and_between_values(dtype, code, G, T):
         x[:, :, zeros] = 0.0
         out, kd, vd = run(q, k, x, mask, None, code)
         close(out, q, kd, vd, mask, [L], 128 ** -0.5, True)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("G,T,D", [(4, 3, 128), (4, 8, 128), (4, 8, 64), (8, 40, 128), (8, 40, 64)])
+@pytest.mark.parametrize("generic", [False, True])
+def test_nan_codes_reach_their_column_of_the_rows_that_see_them(dtype, G, T, D, generic):
+    """e4m3 codes 0x7f and 0xff (a cache may come from anywhere) in one element of every drafted value row, and of a row
+    in front of them: the same rule in every kernel."""
+    b, KVH, L = 2, 2, 300
+    lens = [300, max(T - 2, 1)]
+    q, k, v, mask, _ = case(T + D, b, KVH * G, KVH, T, L, D, dtype, "e4m3", "trees")
+    c = K.quantized_cache(b, KVH, L, D, code="e4m3")
+    K.quantized_cache_append(c, k.to(DEV), v.to(DEV), 0)
+    lt = torch.tensor(lens, dtype=torch.int32, device=DEV)
+    kw = dict(force_generic=True) if generic else dict(tcgen05=PIN)
+    call = lambda: K.group_query_attention_quantized(q.to(DEV), c, mask.to(DEV), kv_lens=lt, **kw).cpu()  # noqa: E731
+    held = c.value_codes.view(torch.uint8).cpu()
+    zero, places = scattered(held, lens, T, [0x00])
+    bad, _ = scattered(held, lens, T, [0x7f, 0xff])
+    c.value_codes.view(torch.uint8).copy_(zero)
+    clean = call()
+    want = expected_with(clean, [(i, u, col, float("nan")) for i, u, col, _ in places], mask, T)
+    c.value_codes.view(torch.uint8).copy_(bad)
+    out = call()
+    assert torch.equal(out.isnan(), want.isnan()) and torch.equal(out.nan_to_num(5.0), want.nan_to_num(5.0))
+    assert want.isnan().any() and want.isfinite().any()
+    bad = zero.clone()
+    bad[0, 0, 290 - T, 3] = bad[0, 0, 20, 9] = 0x7f                  # in the drafted rows' tile (or the one before), and far in front
+    c.value_codes.view(torch.uint8).copy_(bad)
+    out = call()
+    assert out[0, :G][..., [3, 9]].isnan().all()
+    out[0, :G, :, 3], out[0, :G, :, 9] = clean[0, :G, :, 3], clean[0, :G, :, 9]
+    assert torch.equal(out, clean)
