@@ -689,3 +689,25 @@ def test_nan_codes_reach_their_column_of_the_rows_that_see_them(dtype, G, T, D, 
     assert out[0, :G][..., [3, 9]].isnan().all()
     out[0, :G, :, 3], out[0, :G, :, 9] = clean[0, :G, :, 3], clean[0, :G, :, 9]
     assert torch.equal(out, clean)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("G,T", [(4, 4), (8, 20)])
+@pytest.mark.parametrize("sign", [1.0, -1.0])
+def test_an_infinite_key_that_a_token_sees(dtype, G, T, sign):
+    """Dense caches, one infinite key element in a row that only the last token sees: a score of +inf makes its output
+    NaN, as inf - inf does in the definition; a score of -inf leaves the row without weight."""
+    L = 300
+    q, k, v, mask, _ = case(T, 1, 2 * G, 2, T, L, 128, dtype, "dense", "tree")
+    q = torch.where(q == 0, torch.ones_like(q), q)
+    mask[:, T - 1] = False
+    hidden, _, _ = run(q, k, v, mask, None, "dense")
+    mask[T - 1, T - 1] = True
+    clean, _, _ = run(q, k, v, mask, None, "dense")
+    k[:, :, L - 1, 40] = sign * float("inf")
+    out, _, _ = run(q, k, v, mask, None, "dense")
+    assert torch.equal(out[:, :, :T - 1], clean[:, :, :T - 1])
+    up = (q[:, :, T - 1, 40] * sign > 0).to(DEV)
+    last = out[:, :, T - 1]
+    assert up.any() and (~up).any()
+    assert last[up].isnan().all() and torch.equal(last[~up], hidden[:, :, T - 1][~up])
