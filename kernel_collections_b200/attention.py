@@ -290,8 +290,10 @@ def _tree_decode(query, idx, KVH, L, k, ks, v, vs, scales, code, tree_mask, sm_s
     """Shared by the two tree entry points: k / v (bsz, KVH, L, head_dim) with strides ks / vs, `scales` the pointers and
     strides of the key and value scales."""
     b, H, T, D = query.shape
-    if H % KVH != 0:
+    if KVH == 0 or H % KVH != 0:
         raise ValueError("num_heads must be divisible by num_kv_heads")
+    if not 0 <= num_splits < 2 ** 31:
+        raise ValueError("num_splits must not be negative")
     tm_ptr, tm_sb, tm_st = 0, 0, 0
     if tree_mask is not None:
         _C.device_index(query, tree_mask)

@@ -123,8 +123,8 @@ def quantized_cache_read(cache, position, length, *, dtype=torch.bfloat16):
     dims, strides = check_cache(cache)
     idx, b, h, cap, d, _ = dims
     n = int(length)
-    if n < 0:
-        raise ValueError("length must not be negative")
+    if not 0 <= n < 2 ** 31:
+        raise ValueError("length must not be negative, and fit 32 bits")
     pos, pos_ptr = _start(position, b, cache.key_codes)
     k = torch.empty((b, h, n, d), dtype=dtype, device=cache.key_codes.device)
     v = torch.empty_like(k)

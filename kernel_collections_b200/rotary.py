@@ -75,7 +75,8 @@ def rotary_embedding(query, key, inv_freq, position, *, interleaved=False, magni
     and `magnitude` from rotary_frequencies.  The first rotary_dim elements of every head are turned, as pairs (j, j +
     rotary_dim / 2) or, with `interleaved`, (2j, 2j + 1); the others are copied.  `position`: an int or an int32
     tensor (bsz,), the position of each sequence's first token with the others following it, or an int32 tensor (bsz,
-    n) of every token's own (drafted trees).  `out`: a (query', key') pair to fill; it may be the inputs themselves."""
+    n) of every token's own (drafted trees).  `out`: a (query', key') pair to fill; it may be the inputs themselves, and share no memory with
+    them otherwise."""
     shape = query.shape
     if len(shape) != 4:
         raise ValueError(f"query must be (bsz, num_heads, n, head_dim); got {tuple(shape)}")
@@ -100,7 +101,7 @@ def rotary_embedding(query, key, inv_freq, position, *, interleaved=False, magni
     if isinstance(position, torch.Tensor):
         _C.device_index(query, position)
         pshape = position.shape
-        if position.dtype != torch.int32 or pshape[0] != b or not (len(pshape) == 1 or (len(pshape) == 2 and pshape[1] == n)):
+        if position.dtype != torch.int32 or not (pshape == (b,) or pshape == (b, n)):
             raise ValueError("positions must be an int32 device tensor of shape (bsz,) or (bsz, n)")
         if len(pshape) == 2:
             position = position.contiguous()
@@ -137,6 +138,9 @@ def rotary_embedding(query, key, inv_freq, position, *, interleaved=False, magni
             _C.device_index(query, o)
             if o.shape != t.shape or o.dtype != dt or (o.stride(3) != 1 and D != 1):
                 raise ValueError("outputs must have the inputs' shapes and dtype and a contiguous last dim")
+            for size, a, c in zip(o.shape, o.stride(), t.stride()):
+                if size > 1 and (a == 0 or (a != c and o.data_ptr() == t.data_ptr())):
+                    raise ValueError("outputs must have an element of memory each, in place exactly the input's")
     if query.numel() == 0:
         if key is not None and key.numel():      # no query heads: the keys turn as the call's only heads
             rotary_embedding(key, None, inv_freq, position, interleaved=interleaved, magnitude=magnitude, out=(ko, None))

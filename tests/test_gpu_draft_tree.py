@@ -711,3 +711,16 @@ def test_an_infinite_key_that_a_token_sees(dtype, G, T, sign):
     last = out[:, :, T - 1]
     assert up.any() and (~up).any()
     assert last[up].isnan().all() and torch.equal(last[~up], hidden[:, :, T - 1][~up])
+
+
+def test_no_key_heads_and_counts_past_32_bits_are_refused():
+    q = torch.zeros(2, 8, 3, 64, dtype=torch.bfloat16, device=DEV)
+    k = torch.zeros(2, 2, 20, 64, dtype=torch.bfloat16, device=DEV)
+    c = K.quantized_cache(2, 2, 20, 64)
+    for kw in [dict(key=k[:, :0], value=k[:, :0]), dict(num_splits=2 ** 31)]:
+        with pytest.raises(ValueError):
+            K.group_query_attention_tree(**{**dict(query=q, key=k, value=k), **kw})
+    with pytest.raises(ValueError):
+        K.group_query_attention_quantized(q, K.quantized_cache(2, 0, 20, 64))
+    with pytest.raises(ValueError):
+        K.quantized_cache_read(c, 0, 2 ** 31)

@@ -159,3 +159,17 @@ def test_keys_alone(interleaved):
     got = K.rotary_embedding(q, k, f, 7, interleaved=interleaved, out=out)
     assert got[0] is out[0] and got[1] is out[1] and torch.equal(out[1], want)
     assert K.rotary_embedding(k, q, f, 7, interleaved=interleaved)[1].shape == q.shape
+
+
+def test_outputs_that_cannot_be_filled_are_refused():
+    """The inputs' memory in another order, memory that several elements share, and a position without a batch."""
+    q, k = inputs(12, 2, 4, 4, 4, 64, torch.bfloat16)
+    f, _ = K.rotary_frequencies(64)
+    one = torch.empty(2, 4, 1, 64, dtype=q.dtype, device=DEV).expand(-1, -1, 4, -1)
+    for kw in [dict(out=(q.transpose(1, 2), torch.empty_like(k))), dict(out=(torch.empty_like(q), k.transpose(1, 2))),
+               dict(out=(one, torch.empty_like(k))), dict(position=torch.zeros((), dtype=torch.int32, device=DEV)),
+               dict(position=torch.zeros(2, 4, 1, dtype=torch.int32, device=DEV))]:
+        before = q.clone(), k.clone()
+        with pytest.raises(ValueError):
+            K.rotary_embedding(**{**dict(query=q, key=k, inv_freq=f, position=0), **kw})
+        assert torch.equal(q, before[0]) and torch.equal(k, before[1])
