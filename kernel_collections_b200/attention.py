@@ -339,7 +339,10 @@ def group_query_attention_tree(query, key, value, tree_mask=None, *, sm_scale=No
     them are the drafted tokens' own, already written: token u in row kv_lens[b] - T + u.  Token t sees every row before
     those, and drafted token u where tree_mask[t, u] (bool, (T, T) or (bsz, T, T); default: u <= t, a chain).  What a
     token does not see does not reach it, NaN and infinities included; a token that sees nothing gives zeros.
-    Logits are multiplied by sm_scale (default 1 / sqrt(head_dim)).  Returns (bsz, num_heads, T, head_dim)."""
+    Logits are multiplied by sm_scale (default 1 / sqrt(head_dim)).  Returns (bsz, num_heads, T, head_dim).
+
+    kv_lens stays on the device, so the kernel is chosen by the cache's capacity (kv_len).  Where every length is known to be
+    far below it, pass views of the rows in use (key[:, :, :n]): the choice then fits them."""
     idx = _C.device_index(query, key, value)
     qshape, shape = query.shape, key.shape
     if len(qshape) != 4 or len(shape) != 4 or shape != value.shape:

@@ -328,7 +328,9 @@ void portable_plan(const xkv_tree_params& p, TreePlan* pl) {
   pl->name = "portable";
   pl->block_rows = RB;
   pl->unit_tokens = UNIT;
-  pl->slots = 4 * device_sm_count();      // about four blocks per SM fit
+  // Four blocks fit an SM over dense caches at head sizes up to 128 (119 registers a thread), three over 8-bit ones (151), two
+  // near head size 256 (86 KB of shared memory): there the last shares run behind the others.
+  pl->slots = 4 * device_sm_count();
 }
 
 bool make_plan(const xkv_tree_params& p, TreePlan* pl) {

@@ -22,10 +22,11 @@
 //    (it cancels in O / l) and go into the product times their value scale, relative to the largest such product: those down
 //    to 2^-20 of it keep all 11 bits, however large the scale of a row without weight may be.
 //  * fp32 queries: Q and P in two fp16 terms each (22 bits), two MMAs instead of one.
-// 4 x 131071 rows of 8 heads (e4m3, 8 query rows per head, 1.1 GB): 173 to 190 us, 5.8 to 6.4 TB/s; the same in int8, with 16 query rows or
-// with fp32 queries within 5 %.  16 ragged sequences of up to 16384 int8 rows (0.42 GB): 78 to
-// 83 us.  One sequence of 777 rows: 13 us,
-// the host's time for the call.
+//  * Over 8-bit caches the reference of the exponents is checked on the products themselves, after they are formed (the few
+//    tiles that move it form them again): no maximum over scores or scales, no exchange between lanes, in the others.
+// Calls queued back to back: 4 x 131071 rows of 8 heads (e4m3, 8 query rows per head, 1.1 GB) 168 to 170 us, 6.5 TB/s; the
+// same in int8 168, with fp32 queries 175 to 179, with 16 query rows 199.  16 ragged sequences of up to 16384 int8 rows (0.42 GB):
+// 74 to 76 us.  One sequence of 777 rows: 13 us, the host's time for the call.
 #include "tree_common.cuh"
 #include "sm100_common.cuh"
 #include <type_traits>
@@ -589,7 +590,7 @@ __global__ void __launch_bounds__(NT, 1) stream_kernel(const Args a) {
       __syncwarp();       // every lane is done with the stage before the next copies into it
     }
 
-    // ---- join the four warps ------------------------------------------------------------------------------------------
+    // ---- join the eight warps ------------------------------------------------------------------------------------------
     asm volatile("cp.async.wait_all;" ::: "memory");
     __syncthreads();
     constexpr int OS = D + 4;

@@ -18,10 +18,14 @@
 // tree_stream_sm100.cu.  P is rounded to the 16-bit type of the product; over 16-bit caches l
 // sums the rounded values.
 // What bounds it.  Per 128 x 128 item the tensor core needs 1024 cycles and the exponentials 1024 of the 16-per-clock unit; a
-// group's chain (softmax 1800, then P.V and S with their latencies 1400) leaves about 2000 per item.  512 fp16 rows over
-// 4 x 32768 rows of 8 heads: 16-bit cache 323 us (852 TFLOP/s), int8 459 us (599: the softmax waits for scales from shared
-// memory).  104 rows over 8 x 16384 ragged bf16 rows: 100 us, steady tiles at the rate of HBM, the rest set-up and ends of the
-// strips.  Handing the exponentials from one group to the other in strict turns was measured slower (536 us against 474).
+// group's chain (softmax 1800, then P.V and S with their latencies 1400) leaves about 2000 per item over 16-bit caches.  Over
+// 8-bit caches it was 3800 when counted: every element takes a key and a value scale from shared memory more, and the softmax
+// does not fit its 144 registers (144 to 284 bytes stored and 396 to 676 loaded per thread as spills; the 16-bit kernels 0 to 16).  What
+// each of the two costs was not separated.  512 fp16 rows over 4 x 32768 rows of 8 heads, calls queued: 16-bit cache 300 us
+// (916 TFLOP/s), int8 440 to 449 (619), e4m3 490 to 494.  104 rows over 8 x 16384 ragged rows: bf16 95 to 101 us, steady tiles at the
+// rate of HBM, the rest set-up and ends of the strips; int8 158 to 160, e4m3 179 to 182 (the scales come with V: the softmax
+// of a tile waits for a widening of V that it does not need yet).  Handing the exponentials from one group to the other in strict turns was
+// measured slower (536 us against 474).
 // All waits are bounded; a group that gives up raises the abort flag, which ends the others' waits.
 #include "tree_common.cuh"
 #include "sm100_common.cuh"
