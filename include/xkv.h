@@ -354,8 +354,10 @@ XKV_API int xkv_cache_read(const xkv_cache_params* p, void* stream);
  *   q   (batch, num_heads, num_tokens, head_dim) of dtype
  *   k,v (batch, num_kv_heads, kv_len, head_dim): of dtype (XKV_CACHE_DENSE), or codes with k_scales / v_scales
  *   out (batch, num_heads * num_tokens, head_dim) of dtype: row h * num_tokens + t at o_sb, o_sr
- * Value scales may differ by any factor between rows: a row counts by its weight times its scale (in full for scales up to
- * 2^112; at 2^121, where a row's largest value ends fp32, the faster kernels lose weights below 2^-11 of the largest).
+ * Over 8-bit caches a row counts by its softmax weight times its value scale.  The two faster kernels keep such products to 11
+ * bits (22 for fp32 queries) down to 2^-20 (2^-9) of the largest that the query row sees and drop those below 2^-31: this shows in
+ * elements in which all larger rows hold zeros.  Value scales up to 2^112; at 2^121, where a row's largest value reaches the end
+ * of fp32, they lose weights below 2^-11 of the largest.  XKV_FLAG_FORCE_GENERIC keeps fp32 throughout.
  * The lengths are on the device, so the kernel is chosen by kv_len, the capacity: a caller who knows that all lengths are far
  * below it passes the smaller kv_len (the strides stay).
  * Flags: XKV_FLAG_FORCE_GENERIC, XKV_FLAG_TREE_TCGEN05, XKV_FLAG_TREE_MMA_SYNC.  head_dim <= 256.  The status words at the
