@@ -24,9 +24,9 @@
 //  * fp32 queries: Q and P in two fp16 terms each (22 bits), two MMAs instead of one.
 //  * Over 8-bit caches the reference of the exponents is checked on the products themselves, after they are formed (the few
 //    tiles that move it form them again): no maximum over scores or scales, no exchange between lanes, in the others.
-// Calls queued back to back: 4 x 131071 rows of 8 heads (e4m3, 8 query rows per head, 1.1 GB) 168 to 170 us, 6.5 TB/s; the
+// Calls queued back to back: 4 x 131071 rows of 8 heads (e4m3, 8 query rows per head, 1.1 GB) 168 to 179 us, 6.2 to 6.6 TB/s, GPU to GPU; the
 // same in int8 168, with fp32 queries 175 to 179, with 16 query rows 199.  16 ragged sequences of up to 16384 int8 rows (0.42 GB):
-// 74 to 76 us.  One sequence of 777 rows: 13 us, the host's time for the call.
+// 74 to 81 us.  One sequence of 777 rows: 13 us, the host's time for the call.
 #include "tree_common.cuh"
 #include "sm100_common.cuh"
 #include <type_traits>

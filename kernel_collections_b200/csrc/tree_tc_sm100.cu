@@ -22,7 +22,7 @@
 // 8-bit caches it was 3800 when counted: every element takes a key and a value scale from shared memory more, and the softmax
 // does not fit its 144 registers (144 to 284 bytes stored and 396 to 676 loaded per thread as spills; the 16-bit kernels 0 to 16).  What
 // each of the two costs was not separated.  512 fp16 rows over 4 x 32768 rows of 8 heads, calls queued: 16-bit cache 300 us
-// (916 TFLOP/s), int8 440 to 449 (619), e4m3 490 to 494.  104 rows over 8 x 16384 ragged rows: bf16 95 to 101 us, steady tiles at the
+// (916 TFLOP/s), int8 440 to 457 (600 to 625), e4m3 490 to 494.  104 rows over 8 x 16384 ragged rows: bf16 95 to 105 us, steady tiles at the
 // rate of HBM, the rest set-up and ends of the strips; int8 158 to 160, e4m3 179 to 182 (the scales come with V: the softmax
 // of a tile waits for a widening of V that it does not need yet).  Handing the exponentials from one group to the other in strict turns was
 // measured slower (536 us against 474).
